@@ -310,9 +310,93 @@ qsamp_status qsamp_verify_greedy(qsamp_ctx* ctx, const void* logits, qsamp_dtype
                                  int32_t eos_token, int32_t* out_accepted, int32_t* out_bonus,
                                  int32_t* out_has_bonus, void* stream);
 
+/* The output head around the selection. -----------------------------------
+ * No counterpart in the reference (its head is a graph op, its sampler ends
+ * at the token). All of it is stream-ordered on `stream`, needs no device
+ * allocation, may be captured into a CUDA graph, and gives the same bits for
+ * the same call every time. Buffers are DEVICE memory, borrowed for the call;
+ * outputs must not overlap inputs or the workspace. The workspace belongs to
+ * the caller, 256-byte aligned: two calls that may overlap on the GPU (two
+ * streams, two captured graphs) need one each. A bounded wait that ran out
+ * in one of these kernels is reported by qsamp_poll_status (QSAMP_ERR_DEVICE,
+ * once); the outputs of the calls since the last report are then invalid.
+ *
+ * Cross entropy of N hidden rows under a head weight, without the [N][V]
+ * logits in memory:
+ *   z[n][v]  = hidden[n] . weight[v],  l = z, or softcap * tanh(z / softcap)
+ *   lse[n]   = log sum_v exp l[n][v],  loss[n] = lse[n] - l[n][targets[n]]
+ * A row with a negative target has loss 0 and no gradient (its lse is still
+ * written); a target >= V gives loss NaN and no gradient. -loss is the
+ * token's log-probability (logprobs of generated tokens, prompt scoring).
+ * A logit of +infinity or NaN makes its row's results NaN.
+ *
+ * qsamp_head_loss_grad takes the lse of the forward call on the same inputs
+ * and grad_loss[n] = d(total) / d(loss[n]):
+ *   dz[n][v] = grad_loss[n] (exp(l - lse) - [v = target]) (1 - (l / softcap)^2)
+ *   d_hidden = dz weight,  d_weight = dz^T hidden
+ * (the last factor only with a soft-cap). dz is made again in pieces of the
+ * vocabulary and rounded to bf16, the products' type; sums and d_hidden
+ * across pieces are held in 32 bits; both gradients are rounded to bf16 once
+ * at the end and overwrite their buffers. grad_loss is not read for rows
+ * without a gradient.
+ *
+ * bf16 matrices; D, every stride a multiple of 8 elements and every matrix
+ * 16-byte aligned (else QSAMP_ERR_UNSUPPORTED). N = 0 is served (d_weight = 0).
+ * qsamp_head_workspace: bytes either call needs for N rows (grad = 0: the
+ * loss, 1: the gradients), -1 on an invalid argument. */
+typedef struct qsamp_head {
+    const void* hidden;      /* DEVICE bf16 [N][hidden_stride]   */
+    const void* weight;      /* DEVICE bf16 [V][weight_stride]   */
+    const int32_t* targets;  /* DEVICE [N]                       */
+    int32_t N, V, D;
+    int64_t hidden_stride, weight_stride; /* elements, >= D      */
+    float softcap;           /* 0: off                           */
+} qsamp_head;
+int64_t qsamp_head_workspace(const qsamp_ctx* ctx, int32_t N, int32_t V, int32_t D, int32_t grad);
+qsamp_status qsamp_head_loss(qsamp_ctx* ctx, const qsamp_head* head, float* out_loss, float* out_lse, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+qsamp_status qsamp_head_loss_grad(qsamp_ctx* ctx, const qsamp_head* head, const float* lse, const float* grad_loss,
+                                  void* d_hidden, int64_t d_hidden_stride, void* d_weight, int64_t d_weight_stride,
+                                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* 8-bit floating point (e4m3) with a scale for each block of 128.
+ *
+ * qsamp_quantize_fp8: x (fp32 or bf16 [M][x_stride]) in blocks of block_rows
+ * x 128 elements, block_rows 1 (activations) or 128 (weights), short blocks
+ * at the ends: scale = amax / 448 rounded to 32 bits, q = x / scale rounded
+ * once to e4m3 (ties to even, saturating at 448); a block of zeros has scale
+ * 0 and q 0; a block holding an infinity or a NaN has a NaN scale and NaN q.
+ * scale is [ceil(M / block_rows)][scale_stride]. Any stride >= K and any
+ * alignment of x and q is served.
+ *
+ * qsamp_matmul_fp8: out[m][n] = sum over blocks kb of 128 of
+ *   x_scale[m][kb] * w_scale[n / 128][kb] * (x[m] . w[n] within the block),
+ * x [M][x_stride] with a scale per row and block, w [V][w_stride] with a scale
+ * per 128 x 128 block: the head's logits for qsamp_sample (or any linear
+ * layer). Products within a block and the sum over blocks are held in 32
+ * bits; out is fp32 or bf16, rounded once. x and w 16-byte aligned with
+ * strides a multiple of 16 (else QSAMP_ERR_UNSUPPORTED); K, M and V any size;
+ * out any alignment of its type and any stride >= V. */
+typedef struct qsamp_fp8_product {
+    const void* x;           /* DEVICE e4m3 [M][x_stride]                */
+    const float* x_scale;    /* DEVICE [M][x_scale_stride]               */
+    const void* w;           /* DEVICE e4m3 [V][w_stride]                */
+    const float* w_scale;    /* DEVICE [ceil(V / 128)][w_scale_stride]   */
+    int32_t M, V, K;
+    int64_t x_stride, x_scale_stride, w_stride, w_scale_stride;
+    void* out;               /* DEVICE [M][out_stride] of out_dtype      */
+    qsamp_dtype out_dtype;
+    int64_t out_stride;
+} qsamp_fp8_product;
+qsamp_status qsamp_quantize_fp8(qsamp_ctx* ctx, const void* x, qsamp_dtype dtype, int32_t M, int32_t K,
+                                int64_t x_stride, int32_t block_rows, void* q, int64_t q_stride, float* scale,
+                                int64_t scale_stride, void* stream);
+qsamp_status qsamp_matmul_fp8(qsamp_ctx* ctx, const qsamp_fp8_product* p, void* stream);
+
 /* Counters since creation (observability). No counterpart in the
  * reference. kernel_launches counts every kernel this context launched
- * (selection, merge, soft-cap tables). With kernel timing on, each selection
+ * (selection, merge, soft-cap tables, verification, masks, output head).
+ * With kernel timing on, each selection
  * kernel launch is bracketed by CUDA events on the call's stream and
  * qsamp_get_counters waits for the last call's events and reports their
  * device times (0 for a kernel the call did not launch); timing off (the

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "qsamp_device.h"
+#include "qsamp_head.h"
 
 extern "C" cudaError_t qs_launch_rows(const qs::QsLaunch* a, int clusters, int cl, size_t smem, cudaStream_t st);
 extern "C" cudaError_t qs_kernel_attrs(size_t smem);
@@ -111,6 +112,10 @@ struct qsamp_ctx {
     // the device status word of the last asynchronous call, copied here in
     // stream order at the end of the call (qsamp_poll_status reads it)
     int* pinned_status = nullptr;
+    // mapped host word the output-head kernels write when a bounded wait runs
+    // out (they have no per-call status to clear or copy); read and cleared by
+    // qsamp_poll_status
+    int* head_status = nullptr;
     // device-side bounds (qsamp_set_limits)
     int max_rounds = kMaxRounds;
     unsigned long long ready_wait_ns = 1000000000ull;
@@ -416,6 +421,8 @@ qsamp_status qsamp_create(int32_t device, qsamp_ctx** out) {
     if (e == cudaSuccess) *c->pinned_one = 1;
     if (e == cudaSuccess) e = cudaHostAlloc((void**)&c->pinned_status, 8 * sizeof(int), cudaHostAllocDefault);
     if (e == cudaSuccess) std::memset(c->pinned_status, 0, 8 * sizeof(int));
+    if (e == cudaSuccess) e = cudaHostAlloc((void**)&c->head_status, sizeof(int), cudaHostAllocMapped);
+    if (e == cudaSuccess) *c->head_status = 0;
     cudaSetDevice(prev);
     if (e != cudaSuccess) {
         qsamp_destroy(c);  // releases whatever was created
@@ -451,6 +458,7 @@ void qsamp_destroy(qsamp_ctx* c) {
     c->vparts.release();
     if (c->pinned_one) cudaFreeHost(c->pinned_one);
     if (c->pinned_status) cudaFreeHost(c->pinned_status);
+    if (c->head_status) cudaFreeHost(c->head_status);
     if (c->copy_go) cudaEventDestroy(c->copy_go);
     if (c->copy_done) cudaEventDestroy(c->copy_done);
     if (c->copy) cudaStreamDestroy(c->copy);
@@ -912,6 +920,12 @@ qsamp_status qsamp_sample_host(qsamp_ctx* c, const qsamp_batch* hb) {
 qsamp_status qsamp_poll_status(qsamp_ctx* c) {
     if (!c) return QSAMP_ERR_INVALID_ARG;
     std::lock_guard<std::mutex> g(c->mu);
+    volatile int* head = c->head_status;
+    if (*head != 0) {
+        *head = 0;
+        return fail(c, QSAMP_ERR_DEVICE,
+                    "device: a bounded wait ran out in an output-head kernel (its outputs are invalid)");
+    }
     return status_of(c, *(volatile int*)c->pinned_status);
 }
 
@@ -1296,6 +1310,201 @@ qsamp_status qsamp_merge_topk(qsamp_ctx* c, int32_t n_ranks, int32_t B, int32_t 
                                   (cudaStream_t)stream);
     if (prev != c->device) cudaSetDevice(prev);
     return s;
+}
+
+// ---------------------------------------------------------------- output head
+int64_t qsamp_head_workspace(const qsamp_ctx* c, int32_t N, int32_t V, int32_t D, int32_t grad) {
+    if (!c || N < 0 || V < 1 || D < 1) return -1;
+    return grad ? qs_head_grad_ws(N, V, D, c->num_sms) : qs_head_loss_ws(N, V, D, c->num_sms);
+}
+
+// A matrix the tensor copies read: base and rows on 16-byte boundaries.
+static qsamp_status check_matrix(qsamp_ctx* c, const char* name, const void* p, int64_t stride, int64_t least, int esz) {
+    if (stride < least)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "%s stride: expected >= %lld, got %lld", name, (long long)least,
+                    (long long)stride);
+    if ((uintptr_t)p % 16 != 0)
+        return fail(c, QSAMP_ERR_UNSUPPORTED, "%s: expected 16-byte alignment, got address %p", name, p);
+    if (stride % (16 / esz) != 0)
+        return fail(c, QSAMP_ERR_UNSUPPORTED, "%s stride: expected a multiple of %d elements, got %lld", name, 16 / esz,
+                    (long long)stride);
+    if (stride >= (int64_t(1) << 39) / esz)
+        return fail(c, QSAMP_ERR_UNSUPPORTED, "%s stride: expected rows below 2^39 bytes, got %lld elements", name,
+                    (long long)stride);
+    return QSAMP_OK;
+}
+
+// Tiles are numbered in 32 bits.
+static qsamp_status check_tiles(qsamp_ctx* c, int64_t rows, int64_t cols) {
+    if (((rows + 63) / 64) * ((cols + 63) / 64) > INT32_MAX)
+        return fail(c, QSAMP_ERR_UNSUPPORTED, "a result of %lld x %lld: more tiles than one call numbers",
+                    (long long)rows, (long long)cols);
+    return QSAMP_OK;
+}
+
+static qsamp_status head_call(qsamp_ctx* c, const qsamp_head* h, int grad, void* workspace, int64_t workspace_bytes,
+                              qs::HeadCall& a) {
+    if (!h) return fail(c, QSAMP_ERR_INVALID_ARG, "head: expected non-NULL");
+    if (h->N < 0) return fail(c, QSAMP_ERR_INVALID_ARG, "N: expected >= 0, got %d", h->N);
+    if (h->V < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "V: expected >= 1, got %d", h->V);
+    if (h->D < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "D: expected >= 1, got %d", h->D);
+    if (h->D % 8 != 0) return fail(c, QSAMP_ERR_UNSUPPORTED, "D: expected a multiple of 8, got %d", h->D);
+    if (!(h->softcap >= 0.0f) || std::isinf(h->softcap))
+        return fail(c, QSAMP_ERR_INVALID_ARG, "softcap: expected a number >= 0, got %g", h->softcap);
+    if (!h->weight) return fail(c, QSAMP_ERR_INVALID_ARG, "weight: expected non-NULL");
+    if (h->N > 0 && (!h->hidden || !h->targets))
+        return fail(c, QSAMP_ERR_INVALID_ARG, "hidden / targets: expected non-NULL");
+    qsamp_status s = check_matrix(c, "hidden", h->hidden, h->hidden_stride, h->D, 2);
+    if (s == QSAMP_OK) s = check_matrix(c, "weight", h->weight, h->weight_stride, h->D, 2);
+    if (s == QSAMP_OK) s = check_tiles(c, h->N, h->V);
+    if (s == QSAMP_OK) s = check_tiles(c, h->N, h->D);
+    if (s == QSAMP_OK) s = check_tiles(c, h->V, h->D);
+    if (s != QSAMP_OK) return s;
+    const int64_t need = qsamp_head_workspace(c, h->N, h->V, h->D, grad);
+    if (need > 0 && !workspace) return fail(c, QSAMP_ERR_INVALID_ARG, "workspace: expected non-NULL");
+    if (workspace_bytes < need)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "workspace_bytes: expected >= %lld, got %lld", (long long)need,
+                    (long long)workspace_bytes);
+    if ((uintptr_t)workspace % 256 != 0)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "workspace: expected 256-byte alignment, got address %p", workspace);
+    a = qs::HeadCall{};
+    a.hidden = (const uint16_t*)h->hidden;
+    a.weight = (const uint16_t*)h->weight;
+    a.targets = h->targets;
+    a.N = h->N;
+    a.V = h->V;
+    a.D = h->D;
+    a.hidden_stride = h->hidden_stride;
+    a.weight_stride = h->weight_stride;
+    a.softcap = h->softcap;
+    a.ws = (unsigned char*)workspace;
+    a.num_sms = c->num_sms;
+    a.status = c->head_status;
+    return QSAMP_OK;
+}
+
+}  // extern "C"
+
+// Runs a launch with the context's device current.
+template <typename F>
+static qsamp_status on_device(qsamp_ctx* c, const char* what, F launch) {
+    int prev = 0;
+    cudaGetDevice(&prev);
+    if (prev != c->device) cudaSetDevice(c->device);
+    int launches = 0;
+    const cudaError_t e = launch(&launches);
+    if (prev != c->device) cudaSetDevice(prev);
+    c->ctr.kernel_launches += launches;
+    return e == cudaSuccess ? QSAMP_OK : cuda_fail(c, e, what);
+}
+
+extern "C" {
+
+qsamp_status qsamp_head_loss(qsamp_ctx* c, const qsamp_head* head, float* out_loss, float* out_lse, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+    if (!c) return QSAMP_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> g(c->mu);
+    qs::HeadCall a;
+    const qsamp_status s = head_call(c, head, 0, workspace, workspace_bytes, a);
+    if (s != QSAMP_OK) return s;
+    if (a.N == 0) return QSAMP_OK;
+    if (!out_loss || !out_lse) return fail(c, QSAMP_ERR_INVALID_ARG, "out_loss / out_lse: expected non-NULL");
+    a.loss = out_loss;
+    a.lse_out = out_lse;
+    return on_device(c, "head loss launch", [&](int* n) { return qs_head_loss(&a, n, (cudaStream_t)stream); });
+}
+
+qsamp_status qsamp_head_loss_grad(qsamp_ctx* c, const qsamp_head* head, const float* lse, const float* grad_loss,
+                                  void* d_hidden, int64_t d_hidden_stride, void* d_weight, int64_t d_weight_stride,
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!c) return QSAMP_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> g(c->mu);
+    qs::HeadCall a;
+    qsamp_status s = head_call(c, head, 1, workspace, workspace_bytes, a);
+    if (s != QSAMP_OK) return s;
+    if (a.N > 0 && (!lse || !grad_loss || !d_hidden))
+        return fail(c, QSAMP_ERR_INVALID_ARG, "lse / grad_loss / d_hidden: expected non-NULL");
+    if (!d_weight) return fail(c, QSAMP_ERR_INVALID_ARG, "d_weight: expected non-NULL");
+    s = check_matrix(c, "d_hidden", d_hidden, d_hidden_stride, a.D, 2);
+    if (s == QSAMP_OK) s = check_matrix(c, "d_weight", d_weight, d_weight_stride, a.D, 2);
+    if (s != QSAMP_OK) return s;
+    a.lse = lse;
+    a.grad_loss = grad_loss;
+    a.d_hidden = (uint16_t*)d_hidden;
+    a.d_weight = (uint16_t*)d_weight;
+    a.d_hidden_stride = d_hidden_stride;
+    a.d_weight_stride = d_weight_stride;
+    return on_device(c, "head gradient launch", [&](int* n) { return qs_head_grad(&a, n, (cudaStream_t)stream); });
+}
+
+qsamp_status qsamp_quantize_fp8(qsamp_ctx* c, const void* x, qsamp_dtype dtype, int32_t M, int32_t K, int64_t x_stride,
+                                int32_t block_rows, void* q, int64_t q_stride, float* scale, int64_t scale_stride,
+                                void* stream) {
+    if (!c) return QSAMP_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> g(c->mu);
+    if (dtype != QSAMP_F32 && dtype != QSAMP_BF16)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "dtype: expected QSAMP_F32 or QSAMP_BF16, got %d", (int)dtype);
+    if (M < 0) return fail(c, QSAMP_ERR_INVALID_ARG, "M: expected >= 0, got %d", M);
+    if (K < 1 || K > 65535 * qs::FP8_BLOCK)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "K: expected [1,%d], got %d", 65535 * qs::FP8_BLOCK, K);
+    if (block_rows != 1 && block_rows != qs::FP8_BLOCK)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "block_rows: expected 1 or %d, got %d", qs::FP8_BLOCK, block_rows);
+    const int64_t kb = qs::ceil_div(K, qs::FP8_BLOCK);
+    if (x_stride < K || q_stride < K || scale_stride < kb)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "x / q / scale stride: expected >= %d / %d / %lld, got %lld / %lld / %lld", K,
+                    K, (long long)kb, (long long)x_stride, (long long)q_stride, (long long)scale_stride);
+    if (M == 0) return QSAMP_OK;
+    if (!x || !q || !scale) return fail(c, QSAMP_ERR_INVALID_ARG, "x / q / scale: expected non-NULL");
+    return on_device(c, "quantisation launch", [&](int* n) {
+        *n = 1;
+        return qs_quantize_fp8(x, (int)dtype, M, K, x_stride, block_rows, (uint8_t*)q, q_stride, scale, scale_stride,
+                               (cudaStream_t)stream);
+    });
+}
+
+qsamp_status qsamp_matmul_fp8(qsamp_ctx* c, const qsamp_fp8_product* p, void* stream) {
+    if (!c) return QSAMP_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> g(c->mu);
+    if (!p) return fail(c, QSAMP_ERR_INVALID_ARG, "product: expected non-NULL");
+    if (p->M < 0) return fail(c, QSAMP_ERR_INVALID_ARG, "M: expected >= 0, got %d", p->M);
+    if (p->V < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "V: expected >= 1, got %d", p->V);
+    if (p->K < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "K: expected >= 1, got %d", p->K);
+    if (p->out_dtype != QSAMP_F32 && p->out_dtype != QSAMP_BF16)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "out_dtype: expected QSAMP_F32 or QSAMP_BF16, got %d", (int)p->out_dtype);
+    const int64_t kb = qs::ceil_div(p->K, qs::FP8_BLOCK);
+    if (p->x_scale_stride < kb || p->w_scale_stride < kb)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "x_scale / w_scale stride: expected >= %lld, got %lld / %lld", (long long)kb,
+                    (long long)p->x_scale_stride, (long long)p->w_scale_stride);
+    if (p->out_stride < p->V)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "out_stride: expected >= V (%d), got %lld", p->V, (long long)p->out_stride);
+    if (p->M == 0) return QSAMP_OK;
+    if (!p->x || !p->w || !p->x_scale || !p->w_scale || !p->out)
+        return fail(c, QSAMP_ERR_INVALID_ARG, "x / w / x_scale / w_scale / out: expected non-NULL");
+    qsamp_status s = check_matrix(c, "x", p->x, p->x_stride, p->K, 1);
+    if (s == QSAMP_OK) s = check_matrix(c, "w", p->w, p->w_stride, p->K, 1);
+    if (s == QSAMP_OK) s = check_tiles(c, p->M, p->V);
+    if (s != QSAMP_OK) return s;
+    qs::Fp8Call a = {};
+    a.x = (const uint8_t*)p->x;
+    a.w = (const uint8_t*)p->w;
+    a.sx = p->x_scale;
+    a.sw = p->w_scale;
+    a.out = p->out;
+    a.M = p->M;
+    a.V = p->V;
+    a.K = p->K;
+    a.out_bf16 = p->out_dtype == QSAMP_BF16;
+    a.x_stride = p->x_stride;
+    a.w_stride = p->w_stride;
+    a.sx_stride = p->x_scale_stride;
+    a.sw_stride = p->w_scale_stride;
+    a.out_stride = p->out_stride;
+    a.num_sms = c->num_sms;
+    a.status = c->head_status;
+    return on_device(c, "8-bit product launch", [&](int* n) {
+        *n = 1;
+        return qs_matmul_fp8(&a, (cudaStream_t)stream);
+    });
 }
 
 }  // extern "C"

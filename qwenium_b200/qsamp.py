@@ -13,6 +13,7 @@ sampling.cpp:101,140. ``Context.sample_batch`` is the batched device entry.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional, Sequence
@@ -69,6 +70,7 @@ EXPORTS = (
     "qsamp_trie_build", "qsamp_trie_free", "qsamp_trie_token_count", "qsamp_trie_memory_bytes",
     "qsamp_trie_collect_by_prefix", "qsamp_trie_collect_by_char_class", "qsamp_trie_collect_by_first_char",
     "qsamp_trie_mark_char_class",
+    "qsamp_head_workspace", "qsamp_head_loss", "qsamp_head_loss_grad", "qsamp_quantize_fp8", "qsamp_matmul_fp8",
 )
 
 _P = ctypes.c_void_p
@@ -136,6 +138,39 @@ class _Limits(ctypes.Structure):
         ("ready_wait_ns", ctypes.c_int64),
         ("hist_path", ctypes.c_int32),
         ("live_path", ctypes.c_int32),
+    ]
+
+
+class _Head(ctypes.Structure):
+    _fields_ = [
+        ("hidden", _P),
+        ("weight", _P),
+        ("targets", _P),
+        ("N", ctypes.c_int32),
+        ("V", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("hidden_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("softcap", ctypes.c_float),
+    ]
+
+
+class _Fp8Product(ctypes.Structure):
+    _fields_ = [
+        ("x", _P),
+        ("x_scale", _P),
+        ("w", _P),
+        ("w_scale", _P),
+        ("M", ctypes.c_int32),
+        ("V", ctypes.c_int32),
+        ("K", ctypes.c_int32),
+        ("x_stride", ctypes.c_int64),
+        ("x_scale_stride", ctypes.c_int64),
+        ("w_stride", ctypes.c_int64),
+        ("w_scale_stride", ctypes.c_int64),
+        ("out", _P),
+        ("out_dtype", ctypes.c_int),
+        ("out_stride", ctypes.c_int64),
     ]
 
 
@@ -213,6 +248,18 @@ def load(path: str = LIB_PATH):
     lib.qsamp_trie_collect_by_first_char.argtypes = [_P, ctypes.c_uint8, _P, ctypes.c_int64]
     lib.qsamp_trie_mark_char_class.restype = ctypes.c_int
     lib.qsamp_trie_mark_char_class.argtypes = [_P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P]
+    lib.qsamp_head_workspace.restype = ctypes.c_int64
+    lib.qsamp_head_workspace.argtypes = [_P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
+    lib.qsamp_head_loss.restype = ctypes.c_int
+    lib.qsamp_head_loss.argtypes = [_P, ctypes.POINTER(_Head), _P, _P, _P, ctypes.c_int64, _P]
+    lib.qsamp_head_loss_grad.restype = ctypes.c_int
+    lib.qsamp_head_loss_grad.argtypes = [_P, ctypes.POINTER(_Head), _P, _P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P,
+                                         ctypes.c_int64, _P]
+    lib.qsamp_quantize_fp8.restype = ctypes.c_int
+    lib.qsamp_quantize_fp8.argtypes = [_P, _P, ctypes.c_int, ctypes.c_int32, ctypes.c_int32, ctypes.c_int64,
+                                       ctypes.c_int32, _P, ctypes.c_int64, _P, ctypes.c_int64, _P]
+    lib.qsamp_matmul_fp8.restype = ctypes.c_int
+    lib.qsamp_matmul_fp8.argtypes = [_P, ctypes.POINTER(_Fp8Product), _P]
     _lib = lib
     return lib
 
@@ -544,6 +591,143 @@ class Context:
         else:
             self._check(rc, "qsamp_sample_host")
         return ids, res, top_ids, top_probs
+
+
+    # ------------------------------------------------------------ output head
+    def _on(self, stream):
+        """(raw stream, a context in which torch allocates for that stream):
+        `stream`, or torch's current stream of this context's device."""
+        import torch
+
+        if stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream, contextlib.nullcontext()
+        return int(stream), torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=self.device))
+
+    def _tensor(self, name, t, dtypes, shape):
+        """Checks a CUDA tensor argument: its dtype, its shape (None: any
+        size), this context's device, unit stride in the last dimension."""
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise QsampError(1, f"{name}: expected a tensor on cuda:{self.device}, got {t.device}")
+        if t.dtype not in dtypes:
+            raise QsampError(1, f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
+        if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+            raise QsampError(1, f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise QsampError(1, f"{name}: expected unit stride in the last dimension, got {t.stride()}")
+
+    @staticmethod
+    def _row_stride(t):
+        """Elements between rows; a single row's stride is free."""
+        return int(t.stride(0)) if t.shape[0] > 1 else -(-int(t.shape[1]) // 16) * 16
+
+    def _head(self, hidden, weight, targets, softcap):
+        import torch
+
+        self._tensor("hidden", hidden, (torch.bfloat16,), (None, None))
+        N, D = (int(x) for x in hidden.shape)
+        self._tensor("weight", weight, (torch.bfloat16,), (None, D))
+        self._tensor("targets", targets, (torch.int32,), (N,))
+        h = _Head(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), N, int(weight.shape[0]), D,
+                  self._row_stride(hidden), self._row_stride(weight), float(softcap))
+        return h
+
+    def _workspace(self, h, grad):
+        import torch
+
+        n = self.lib.qsamp_head_workspace(self.h, h.N, h.V, h.D, grad)
+        if n < 0:
+            raise QsampError(1, f"head: expected N >= 0, V >= 1, D >= 1, got {h.N}, {h.V}, {h.D}")
+        return torch.empty(n, dtype=torch.uint8, device=f"cuda:{self.device}")
+
+    def head_loss(self, hidden, weight, targets, softcap: float = 0.0, stream=None):
+        """qsamp_head_loss on CUDA tensors: hidden bf16 [N][D], weight bf16
+        [V][D], targets int32 [N] (negative: no loss for the row). Returns
+        (loss, lse) float32 [N]; -loss is each target's log-probability."""
+        import torch
+
+        h = self._head(hidden, weight, targets, softcap)
+        raw, alloc = self._on(stream)
+        with alloc:
+            ws = self._workspace(h, 0)
+            out = torch.empty((2, h.N), dtype=torch.float32, device=hidden.device)
+        loss, lse = out[0], out[1]
+        self._check(self.lib.qsamp_head_loss(self.h, ctypes.byref(h), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(),
+                                             ws.numel(), raw), "qsamp_head_loss")
+        return loss, lse
+
+    def head_loss_grad(self, hidden, weight, targets, lse, grad_loss, softcap: float = 0.0, d_hidden=None,
+                       d_weight=None, stream=None):
+        """qsamp_head_loss_grad on CUDA tensors: the inputs of head_loss, its
+        lse, and grad_loss float32 [N] = d(total) / d(loss). Returns
+        (d_hidden, d_weight) bf16, written into the given tensors if any."""
+        import torch
+
+        h = self._head(hidden, weight, targets, softcap)
+        self._tensor("lse", lse, (torch.float32,), (h.N,))
+        self._tensor("grad_loss", grad_loss, (torch.float32,), (h.N,))
+        raw, alloc = self._on(stream)
+        with alloc:
+            ws = self._workspace(h, 1)
+            if d_hidden is None:
+                d_hidden = torch.empty((h.N, h.D), dtype=torch.bfloat16, device=hidden.device)
+            if d_weight is None:
+                d_weight = torch.empty((h.V, h.D), dtype=torch.bfloat16, device=hidden.device)
+        self._tensor("d_hidden", d_hidden, (torch.bfloat16,), (h.N, h.D))
+        self._tensor("d_weight", d_weight, (torch.bfloat16,), (h.V, h.D))
+        self._check(self.lib.qsamp_head_loss_grad(self.h, ctypes.byref(h), lse.data_ptr(), grad_loss.data_ptr(),
+                                                  d_hidden.data_ptr(), self._row_stride(d_hidden),
+                                                  d_weight.data_ptr(), self._row_stride(d_weight), ws.data_ptr(),
+                                                  ws.numel(), raw), "qsamp_head_loss_grad")
+        return d_hidden, d_weight
+
+    def quantize_fp8(self, x, block_rows: int = 1, stream=None):
+        """qsamp_quantize_fp8 on a CUDA tensor x (float32 or bfloat16 [M][K]).
+        Returns (q float8_e4m3fn [M][K], scale float32 [ceil(M/block_rows)]
+        [ceil(K/128)]); q's rows are padded to a multiple of 16 bytes, as
+        matmul_fp8 reads them. block_rows: 1 (activations) or 128 (weights)."""
+        import torch
+
+        self._tensor("x", x, (torch.float32, torch.bfloat16), (None, None))
+        if block_rows not in (1, 128):
+            raise QsampError(1, f"block_rows: expected 1 or 128, got {block_rows}")
+        M, K = (int(v) for v in x.shape)
+        kb = -(-K // 128)
+        raw, alloc = self._on(stream)
+        with alloc:
+            q = torch.empty((M, -(-K // 16) * 16), dtype=torch.float8_e4m3fn, device=x.device)[:, :K]
+            scale = torch.empty((-(-M // block_rows), kb), dtype=torch.float32, device=x.device)
+        self._check(self.lib.qsamp_quantize_fp8(self.h, x.data_ptr(), QSAMP_BF16 if x.dtype == torch.bfloat16 else QSAMP_F32,
+                                                M, K, self._row_stride(x), int(block_rows), q.data_ptr(),
+                                                self._row_stride(q), scale.data_ptr(), max(kb, 1), raw),
+                    "qsamp_quantize_fp8")
+        return q, scale
+
+    def matmul_fp8(self, x, x_scale, w, w_scale, out=None, out_dtype=None, stream=None):
+        """qsamp_matmul_fp8 on CUDA tensors: x float8_e4m3fn [M][K] with
+        x_scale float32 [M][ceil(K/128)], w float8_e4m3fn [V][K] with w_scale
+        float32 [ceil(V/128)][ceil(K/128)]. Returns out [M][V], bfloat16
+        unless `out` or `out_dtype` says float32."""
+        import torch
+
+        self._tensor("x", x, (torch.float8_e4m3fn,), (None, None))
+        M, K = (int(v) for v in x.shape)
+        self._tensor("w", w, (torch.float8_e4m3fn,), (None, K))
+        V, kb = int(w.shape[0]), -(-K // 128)
+        self._tensor("x_scale", x_scale, (torch.float32,), (M, kb))
+        self._tensor("w_scale", w_scale, (torch.float32,), (-(-V // 128), kb))
+        raw, alloc = self._on(stream)
+        if out is None:
+            with alloc:
+                out = torch.empty((M, V), dtype=out_dtype or torch.bfloat16, device=x.device)
+        elif out_dtype is not None and out.dtype != out_dtype:
+            raise QsampError(1, f"out_dtype: expected out's {out.dtype}, got {out_dtype}")
+        self._tensor("out", out, (torch.float32, torch.bfloat16), (M, V))
+        p = _Fp8Product(x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), M, V, K,
+                        self._row_stride(x), self._row_stride(x_scale), self._row_stride(w), self._row_stride(w_scale),
+                        out.data_ptr(), QSAMP_BF16 if out.dtype == torch.bfloat16 else QSAMP_F32,
+                        self._row_stride(out))
+        self._check(self.lib.qsamp_matmul_fp8(self.h, ctypes.byref(p), raw), "qsamp_matmul_fp8")
+        return out
 
 
 # ---------------------------------------------------------------- reference-shaped API
