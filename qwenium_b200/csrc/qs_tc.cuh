@@ -13,6 +13,18 @@ namespace tc {
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// True in one lane of the converged warp. The loops of the loading and the
+// issuing warp run in all lanes and only the instructions themselves in the
+// elected one: the loop's values then stay in uniform registers, which is
+// where tensor copies and matrix instructions take their operands.
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile(
+        "{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}"
+        : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ uint32_t cta_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -38,16 +50,24 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Arrives on a barrier of the cluster (an address from map_to).
+// Arrives on a barrier of this CTA.
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Arrives on a barrier of the cluster (an address from map_to). Relaxed: it
+// only says that tensor memory has been read into registers (tcgen05.wait::ld
+// and the tcgen05 fences order that); a release to the cluster would wait for
+// every store the thread has in flight.
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n.reg .pred p;\n"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         "selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
@@ -69,7 +89,9 @@ constexpr unsigned long long WAIT_NS = 2000000000ull;
 // of this CTA gave up: *gave_up (shared memory) and *status (mapped host
 // memory) are set, and the caller leaves its loop.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
-    if (bar_try(bar, parity)) return true;
+    // the clock is slow to read: the short waits of a running pipeline end before it is
+    for (int spin = 0; spin < 256; ++spin)
+        if (bar_try(bar, parity)) return true;
     const unsigned long long t0 = now_ns();
     for (uint32_t spin = 1;; ++spin) {
         if (bar_try(bar, parity)) return true;
@@ -84,15 +106,29 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     }
 }
 
+// The same for a converged warp: the answer is the warp's.
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, gave_up, status));
+}
+
 // ---------------------------------------------------------------- tensor copies
 // Loads the box at (x, y) into this CTA's shared memory and counts its bytes
-// on `bar`, a barrier of either CTA of the pair (an address from map_to).
+// on `bar`: this CTA's, or with PAIR a barrier of either CTA of the pair (an
+// address from map_to).
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, "
+            "%3}], [%4];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
 }
 
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
@@ -100,13 +136,23 @@ __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
 }
 
 // ---------------------------------------------------------------- tensor memory
+template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    if (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+    if (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -127,8 +173,26 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
         : "r"(addr));
 }
 
-// Until this returns the loaded registers hold nothing; they pass through it
-// so that no use is moved ahead of it.
+// Until tmem_wait_load returns the loaded registers hold nothing; they pass
+// through it so that no use is moved ahead of it.
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+
+__device__ __forceinline__ void tmem_wait_load(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::
+                       "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_load(float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
@@ -148,36 +212,41 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
            (1ull << 46) | (2ull << 61);
 }
 
-// fp32 accumulators, 256 x 256 over the pair; bf16 (kind::f16) or e4m3.
-__host__ __device__ constexpr uint32_t instr_bf16(bool a_mn, bool b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((256u >> 3) << 17) |
-           ((256u >> 4) << 24);
+// fp32 accumulators of m rows and n columns; bf16 (kind::f16) or e4m3.
+__host__ __device__ constexpr uint32_t instr_bf16(int m, int n, bool a_mn, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
 }
-__host__ __device__ constexpr uint32_t instr_e4m3() { return (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24); }
-
-__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
-        : "memory");
+__host__ __device__ constexpr uint32_t instr_e4m3(int m, int n) {
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
-        : "memory");
+#define QS_MMA(group, kind)                                                                        \
+    asm volatile(                                                                                  \
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"                                               \
+        "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n}" ::"r"(d),        \
+        "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)                                             \
+        : "memory")
+template <bool PAIR, bool E4M3>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+    if (PAIR && E4M3) QS_MMA("2", "f8f6f4");
+    if (PAIR && !E4M3) QS_MMA("2", "f16");
+    if (!PAIR && E4M3) QS_MMA("1", "f8f6f4");
+    if (!PAIR && !E4M3) QS_MMA("1", "f16");
 }
+#undef QS_MMA
 
-// The barrier at this offset of both CTAs completes when the matrix
-// instructions issued so far have.
+// The barrier (with PAIR the one at this offset of both CTAs) completes when
+// the matrix instructions issued so far have.
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
-        : "memory");
+    if (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {

@@ -1445,14 +1445,15 @@ qsamp_status qsamp_quantize_fp8(qsamp_ctx* c, const void* x, qsamp_dtype dtype, 
     if (dtype != QSAMP_F32 && dtype != QSAMP_BF16)
         return fail(c, QSAMP_ERR_INVALID_ARG, "dtype: expected QSAMP_F32 or QSAMP_BF16, got %d", (int)dtype);
     if (M < 0) return fail(c, QSAMP_ERR_INVALID_ARG, "M: expected >= 0, got %d", M);
-    if (K < 1 || K > 65535 * qs::FP8_BLOCK)
-        return fail(c, QSAMP_ERR_INVALID_ARG, "K: expected [1,%d], got %d", 65535 * qs::FP8_BLOCK, K);
+    if (K < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "K: expected >= 1, got %d", K);
     if (block_rows != 1 && block_rows != qs::FP8_BLOCK)
         return fail(c, QSAMP_ERR_INVALID_ARG, "block_rows: expected 1 or %d, got %d", qs::FP8_BLOCK, block_rows);
     const int64_t kb = qs::ceil_div(K, qs::FP8_BLOCK);
     if (x_stride < K || q_stride < K || scale_stride < kb)
         return fail(c, QSAMP_ERR_INVALID_ARG, "x / q / scale stride: expected >= %d / %d / %lld, got %lld / %lld / %lld", K,
                     K, (long long)kb, (long long)x_stride, (long long)q_stride, (long long)scale_stride);
+    if ((int64_t)M * kb > (int64_t)INT32_MAX * 8)
+        return fail(c, QSAMP_ERR_UNSUPPORTED, "%d x %d: more blocks than one launch numbers", M, K);
     if (M == 0) return QSAMP_OK;
     if (!x || !q || !scale) return fail(c, QSAMP_ERR_INVALID_ARG, "x / q / scale: expected non-NULL");
     return on_device(c, "quantisation launch", [&](int* n) {

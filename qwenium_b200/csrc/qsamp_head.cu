@@ -49,6 +49,7 @@ struct Params {
     CUtensorMap a, b;    // K contiguous (LSE, DZ, FP8; GRAD: dz for d_hidden)
     CUtensorMap a2, b2;  // GRAD: dz and hidden with K in the rows (d_weight); b: weight with K in the rows
     int m_tiles, n_tiles, k_blocks, jobs;
+    int slice;           // K blocks summed in tensor memory before the epilogue takes them
     int M, N;            // rows of the left and right operand
     int* status;
     // LSE / DZ
@@ -74,6 +75,7 @@ struct Params {
     long long sx_stride, sw_stride, out_stride;
     void* out;
     int out_bf16;
+    int sx_vec;          // rows of sx on 16-byte boundaries
 };
 
 struct Job {
@@ -117,66 +119,63 @@ __device__ __forceinline__ Job job_of(const Params& p, int job) {
 
 // ---------------------------------------------------------------- epilogues
 // One thread's view of a tile: its row, and how to store 32 columns of it.
-__device__ __forceinline__ void logits_of(float (&v)[32], float cap) {
+template <int N>
+__device__ __forceinline__ void logits_of(float (&v)[N], float cap) {
     // cap tanh(z / cap) = cap (1 - 2 / (exp(2 z / cap) + 1)): absolute error a
     // few 2^-24 of cap, and the exponential's overflow gives the limit
     if (cap > 0.0f) {
         const float a = 2.0f * LOG2E / cap;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = cap - 2.0f * cap * __fdividef(1.0f, exp2_approx(v[i] * a) + 1.0f);
+        for (int i = 0; i < N; ++i) v[i] = cap - 2.0f * cap * __fdividef(1.0f, exp2_approx(v[i] * a) + 1.0f);
     }
 }
 
-template <int MODE>
-struct Epilogue;
-
-// Running maximum and sum over the thread's 128 columns, in one pass: 32
-// columns at a time, the sum rescaled when their maximum is larger.
-template <>
-struct Epilogue<LSE> {
-    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, bool live, int target,
-                                float, float) {
-        float mx = -INFINITY, sum = 0.0f, found = 0.0f;
-        bool has = false;
-        const int c0 = j.n0 + half * 128;
-#pragma unroll 1
-        for (int c = 0; c < 128 && c0 + c < p.N; c += 32) {
-            float v[32];
-            tmem_load32(tmem + c, v);
-            tmem_wait_load(v);
-            logits_of(v, p.softcap);
-            const int col = c0 + c;
-            if (col + 32 > p.N) {
+// Running maximum and sum over the thread's 128 columns, 32 at a time, the
+// sum rescaled when their maximum is larger.
+__device__ __forceinline__ void softmax_sums(const Params& p, const Job& j, float (&z)[128], int row, int half, bool live,
+                                             int target) {
+    float mx = -INFINITY, sum = 0.0f, found = 0.0f;
+    bool has = false;
+    const int c0 = j.n0 + half * 128;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (col + i >= p.N) v[i] = -INFINITY;
-            }
-            float m4[4] = {v[0], v[1], v[2], v[3]};
+    for (int c = 0; c < 128; c += 32) {
+        if (c0 + c >= p.N) break;
+        float(&v)[32] = reinterpret_cast<float(&)[32]>(z[c]);
+        logits_of(v, p.softcap);
+        const int col = c0 + c;
+        if (col + 32 > p.N) {
 #pragma unroll
-            for (int i = 4; i < 32; ++i) m4[i % 4] = fmaxf(m4[i % 4], v[i]);
-            const float top = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-            const float ref = top == -INFINITY ? 0.0f : top;
-            float s4[4] = {sum * exp2_approx((mx - ref) * LOG2E), 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s4[i % 4] += exp2_approx((v[i] - ref) * LOG2E);
-            sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            mx = top;
-            if (target >= col && target < col + 32) {
-                has = true;
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (target == col + i) found = v[i];
-            }
+            for (int i = 0; i < 32; ++i)
+                if (col + i >= p.N) v[i] = -INFINITY;
         }
-        if (live) {
-            p.part[(long long)(j.n0 / 128 + half) * p.M + row] = make_float2(mx, sum);
-            if (has) p.target_logit[row] = found;
+        float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int i = 4; i < 32; ++i) m4[i % 4] = fmaxf(m4[i % 4], v[i]);
+        const float top = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float s4[4] = {sum * exp2_approx((mx - ref) * LOG2E), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s4[i % 4] += exp2_approx((v[i] - ref) * LOG2E);
+        sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        mx = top;
+        if (target >= col && target < col + 32) {
+            has = true;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (target == col + i) found = v[i];
         }
     }
-};
+    if (live) {
+        p.part[(long long)(j.n0 / 128 + half) * p.M + row] = make_float2(mx, sum);
+        if (has) p.target_logit[row] = found;
+    }
+}
 
 // dz = g (exp(l - lse) - [target]) (1 - (l / cap)^2), rounded to bf16: the
 // type of the products it goes into. Rows without a gradient are 0.
+template <int MODE>
+struct Epilogue;
+
 template <>
 struct Epilogue<DZ> {
     __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, bool live, int target,
@@ -299,6 +298,13 @@ __device__ __forceinline__ void store_product(const Params& p, const float* v, i
     __syncwarp();
 }
 
+// Scales kb .. kb + 3 of a row; past the end whatever is in reach.
+__device__ __forceinline__ float4 scales4(const float* s, int kb, int n, int vec) {
+    if (kb >= n) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (vec && kb + 4 <= n) return *(const float4*)(s + kb);
+    return make_float4(s[kb], s[min(kb + 1, n - 1)], s[min(kb + 2, n - 1)], s[min(kb + 3, n - 1)]);
+}
+
 // ---------------------------------------------------------------- the kernel
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant__ Params p) {
@@ -325,7 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
         tma_prefetch_map(&p.a);
         tma_prefetch_map(&p.b);
     }
-    if (warp == 1) tmem_alloc(smem_addr(&ctl->tmem), 512);
+    if (warp == 1) tmem_alloc<true>(smem_addr(&ctl->tmem), 512);
     __syncwarp();
     fence_before();
     cluster_sync();
@@ -333,73 +339,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
     const uint32_t tmem = ctl->tmem;
     volatile int* gave_up = &ctl->gave_up;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
         // loads: this CTA's half of both operands, counted on the leader's barrier
         uint32_t it = 0;
         bool ok = true;
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
+            const int m = j.m0 + rank * 128, n = j.n0 + rank * 128;
             for (int kb = 0; kb < j.k_blocks; ++kb, ++it) {
                 const uint32_t s = it % STAGES;
-                if (!(ok = bar_wait(smem_addr(&ctl->empty[s]), (it / STAGES & 1) ^ 1, gave_up, p.status))) break;
-                const uint32_t full = map_to(smem_addr(&ctl->full[s]), 0);
-                if (rank == 0) bar_expect(smem_addr(&ctl->full[s]), 2 * STAGE_BYTES);
-                const uint32_t da = stage0 + s * STAGE_BYTES, db = da + OPERAND_BYTES;
-                const int m = j.m0 + rank * 128, n = j.n0 + rank * 128;
-                if (MODE != GRAD) {
-                    const int x = kb * (MODE == FP8 ? 128 : 64);
-                    tma_load(da, &p.a, x, m, full);
-                    tma_load(db, &p.b, x, n, full);
-                } else {
-                    const int k = (j.k0 + kb) * 64;
-                    if (!j.second) {
-                        tma_load(da, &p.a, k, m, full);
-                        tma_load(db, &p.b, n, p.n0 + k, full);
-                        tma_load(db + OPERAND_BYTES / 2, &p.b, n + 64, p.n0 + k, full);
+                if (!(ok = bar_wait_warp(smem_addr(&ctl->empty[s]), (it / STAGES & 1) ^ 1, gave_up, p.status))) break;
+                if (elected()) {
+                    const uint32_t full = map_to(smem_addr(&ctl->full[s]), 0);
+                    if (rank == 0) bar_expect(smem_addr(&ctl->full[s]), 2 * STAGE_BYTES);
+                    const uint32_t da = stage0 + s * STAGE_BYTES, db = da + OPERAND_BYTES;
+                    if (MODE != GRAD) {
+                        const int x = kb * (MODE == FP8 ? 128 : 64);
+                        tma_load<true>(da, &p.a, x, m, full);
+                        tma_load<true>(db, &p.b, x, n, full);
                     } else {
-                        tma_load(da, &p.a2, m, k, full);
-                        tma_load(da + OPERAND_BYTES / 2, &p.a2, m + 64, k, full);
-                        tma_load(db, &p.b2, n, k, full);
-                        tma_load(db + OPERAND_BYTES / 2, &p.b2, n + 64, k, full);
+                        const int k = (j.k0 + kb) * 64;
+                        if (!j.second) {
+                            tma_load<true>(da, &p.a, k, m, full);
+                            tma_load<true>(db, &p.b, n, p.n0 + k, full);
+                            tma_load<true>(db + OPERAND_BYTES / 2, &p.b, n + 64, p.n0 + k, full);
+                        } else {
+                            tma_load<true>(da, &p.a2, m, k, full);
+                            tma_load<true>(da + OPERAND_BYTES / 2, &p.a2, m + 64, k, full);
+                            tma_load<true>(db, &p.b2, n, k, full);
+                            tma_load<true>(db + OPERAND_BYTES / 2, &p.b2, n + 64, k, full);
+                        }
                     }
                 }
+                __syncwarp();
             }
         }
         // the last stages' releases arrive before this CTA may leave
         for (uint32_t back = it < STAGES ? it : STAGES; ok && back > 0; --back, ++it)
-            ok = bar_wait(smem_addr(&ctl->empty[it % STAGES]), (it / STAGES & 1) ^ 1, gave_up, p.status);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+            ok = bar_wait_warp(smem_addr(&ctl->empty[it % STAGES]), (it / STAGES & 1) ^ 1, gave_up, p.status);
+    } else if (warp == 1 && rank == 0) {
         // matrix instructions: K blocks of 128 bytes, four instructions each
         uint32_t it = 0, acc = 0;
         bool ok = true;
+        const uint64_t op0 = operand(stage0, OPERAND_BYTES / 2);
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
             const bool mn = MODE == GRAD;
-            const uint32_t instr = MODE == FP8 ? instr_e4m3() : instr_bf16(mn && j.second, mn);
+            const uint32_t instr = MODE == FP8 ? instr_e4m3(TILE, TILE) : instr_bf16(TILE, TILE, mn && j.second, mn);
+            // along K: 32 bytes of a row, or 16 rows of 128 bytes (operands count 16 bytes)
+            const uint32_t step_a = (mn && j.second ? 2048 : 32) / 16, step_b = (mn ? 2048 : 32) / 16;
             for (int kb = 0; kb < j.k_blocks; ++kb, ++it) {
-                if (MODE == FP8 || kb == 0) {
-                    if (!(ok = bar_wait(smem_addr(&ctl->acc_empty[acc & 1]), (acc / 2 & 1) ^ 1, gave_up, p.status))) break;
-                }
                 const uint32_t s = it % STAGES;
-                if (!(ok = bar_wait(smem_addr(&ctl->full[s]), it / STAGES & 1, gave_up, p.status))) break;
+                const bool first = kb % p.slice == 0, last = (kb + 1) % p.slice == 0 || kb + 1 == j.k_blocks;
+                if (!(ok = bar_wait_warp(smem_addr(&ctl->full[s]), it / STAGES & 1, gave_up, p.status))) break;
+                if (first && !(ok = bar_wait_warp(smem_addr(&ctl->acc_empty[acc & 1]), (acc / 2 & 1) ^ 1, gave_up, p.status)))
+                    break;
                 fence_after();
-                const uint32_t da = stage0 + s * STAGE_BYTES, db = da + OPERAND_BYTES;
-                const uint32_t d = tmem + (acc & 1) * TILE;
-                // along K: 32 bytes of a row, or 16 rows of 128 bytes
-                const uint32_t step_a = mn && j.second ? 2048 : 32, step_b = mn ? 2048 : 32;
+                if (elected()) {
+                    const uint64_t oa = op0 + s * (STAGE_BYTES / 16), ob = oa + OPERAND_BYTES / 16;
+                    const uint32_t d = tmem + (acc & 1) * TILE;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint64_t oa = operand(da + q * step_a, OPERAND_BYTES / 2);
-                    const uint64_t ob = operand(db + q * step_b, OPERAND_BYTES / 2);
-                    if (MODE == FP8)
-                        mma_e4m3(d, oa, ob, instr, q > 0);
-                    else
-                        mma_bf16(d, oa, ob, instr, kb > 0 || q > 0);
+                    for (int q = 0; q < 4; ++q)
+                        mma<true, MODE == FP8>(d, oa + q * step_a, ob + q * step_b, instr, !first || q > 0);
+                    mma_commit<true>(smem_addr(&ctl->empty[s]));
+                    if (last) mma_commit<true>(smem_addr(&ctl->acc_full[acc & 1]));
                 }
-                mma_commit(smem_addr(&ctl->empty[s]));
-                if (MODE == FP8) mma_commit(smem_addr(&ctl->acc_full[acc++ & 1]));
+                __syncwarp();
+                if (last) ++acc;
             }
-            if (MODE != FP8 && ok) mma_commit(smem_addr(&ctl->acc_full[acc++ & 1]));
         }
     } else if (warp >= 2) {
         const int quarter = warp % 4, half = (warp - 2) / 4;
@@ -409,19 +416,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
             const int row0 = j.m0 + (int)rank * 128 + quarter * 32, row = row0 + lane;
-            if constexpr (MODE != FP8) {
+            if constexpr (MODE == DZ || MODE == GRAD) {
                 const int rows = MODE == GRAD ? (j.second ? p.N : p.rows) : p.M;
                 const bool live = row < rows;
                 int target = -1;
                 float lse = 0.0f, g = 0.0f;
-                if (MODE == LSE && live) target = p.targets[row];
                 if (MODE == DZ && live) {
                     target = p.targets[row];
                     if (target >= p.rows) target = -1;  // DZ: rows holds the vocabulary
                     if (target >= 0) lse = p.lse[row], g = p.grad[row];
                 }
-                ok = bar_wait(smem_addr(&ctl->acc_full[acc & 1]), acc / 2 & 1, gave_up, p.status);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = bar_wait_warp(smem_addr(&ctl->acc_full[acc & 1]), acc / 2 & 1, gave_up, p.status);
                 if (!ok) break;
                 fence_after();
                 if (row0 < rows)
@@ -432,21 +437,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                 if (lane == 0) bar_arrive_cluster(acc & 1 ? empty1 : empty0);
                 ++acc;
             } else {
-                // sum over K blocks of the blocks' own sums times their scales,
-                // in 128 registers
+                // the slices' sums (FP8: a K block each, times its scales) added up in 128 registers
                 float sum[128];
 #pragma unroll
                 for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
                 const bool work = row0 < p.M;
-                const int col = j.n0 + half * 128;
-                const float* sx = p.sx + (row < p.M ? row : 0) * p.sx_stride;
-                const float* sw = p.sw + (col < p.N ? col / 128 : 0) * p.sw_stride;
-                float scale = work ? sx[0] * sw[0] : 0.0f;
-                for (int kb = 0; kb < j.k_blocks; ++kb, ++acc) {
-                    const float now = scale;
-                    if (work && kb + 1 < j.k_blocks) scale = sx[kb + 1] * sw[kb + 1];
-                    ok = bar_wait(smem_addr(&ctl->acc_full[acc & 1]), acc / 2 & 1, gave_up, p.status);
-                    ok = __all_sync(0xffffffffu, ok);
+                const int col = j.n0 + half * 128, slices = (j.k_blocks + p.slice - 1) / p.slice;
+                int target = -1;
+                if (MODE == LSE && row < p.M) target = p.targets[row];
+                // FP8: a row's scales come four K blocks at a time, one group
+                // ahead; a column block's are held by the lanes, 32 K blocks at a time
+                const float* sx = nullptr;
+                const float* sw = nullptr;
+                float4 x4 = {}, next4 = {};
+                float w32 = 0.0f;
+                if (MODE == FP8 && work) {
+                    sx = p.sx + (row < p.M ? row : 0) * p.sx_stride;
+                    sw = p.sw + (col < p.N ? col / 128 : 0) * p.sw_stride;
+                    next4 = scales4(sx, 0, slices, p.sx_vec);
+                }
+                for (int kb = 0; kb < slices; ++kb, ++acc) {
+                    float now = 1.0f;
+                    if (MODE == FP8 && work) {
+                        if (kb % 32 == 0) w32 = sw[min(kb + lane, slices - 1)];
+                        if (kb % 4 == 0) {
+                            x4 = next4;
+                            next4 = scales4(sx, kb + 4, slices, p.sx_vec);
+                        }
+                        const float x = kb % 4 < 2 ? (kb % 4 == 0 ? x4.x : x4.y) : (kb % 4 == 2 ? x4.z : x4.w);
+                        now = x * __shfl_sync(0xffffffffu, w32, kb % 32);
+                    }
+                    ok = bar_wait_warp(smem_addr(&ctl->acc_full[acc & 1]), acc / 2 & 1, gave_up, p.status);
                     if (!ok) break;
                     fence_after();
                     if (work) {
@@ -455,18 +476,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                             float v[32];
                             tmem_load32(tmem + (quarter << 21) + (acc & 1) * TILE + half * 128 + c, v);
                             tmem_wait_load(v);
+                            if (c == 96) {
+                                fence_before();
+                                __syncwarp();
+                                if (lane == 0) bar_arrive_cluster(acc & 1 ? empty1 : empty0);
+                            }
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sum[c + i] = fmaf(v[i], now, sum[c + i]);
+                            for (int i = 0; i < 32; ++i) sum[c + i] = MODE == FP8 ? fmaf(v[i], now, sum[c + i]) : sum[c + i] + v[i];
                         }
+                    } else if (lane == 0) {
+                        bar_arrive_cluster(acc & 1 ? empty1 : empty0);
                     }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive_cluster(acc & 1 ? empty1 : empty0);
                 }
                 if (ok && work) {
+                    if constexpr (MODE == LSE) {
+                        softmax_sums(p, j, sum, row, half, row < p.M, target);
+                    } else {
 #pragma unroll
-                    for (int c = 0; c < 128; c += 32)
-                        if (col + c < p.N) store_product(p, sum + c, row, row0, col + c, patches + (warp - 2) * PATCH_FLOATS);
+                        for (int c = 0; c < 128; c += 32)
+                            if (col + c < p.N)
+                                store_product(p, sum + c, row, row0, col + c, patches + (warp - 2) * PATCH_FLOATS);
+                    }
                 }
             }
         }
@@ -479,9 +509,238 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
     cluster_sync();
     if (warp == 1) {
         fence_after();
-        tmem_free(tmem, 512);
+        tmem_free<true>(tmem, 512);
     }
     cluster_sync();
+}
+
+// ---------------------------------------------------------------- few rows
+// A decode step's rows (at most 128; 32 for the cross entropy) against the
+// whole head: the weight's bytes bound it. Here the weight's rows are the
+// lanes: a CTA multiplies 128 of them by COLS hidden rows at once, so that
+// the matrix instructions cost COLS columns instead of 256, and tensor memory
+// holds 512 / COLS accumulators (up to eight are used), which hides the
+// epilogue's round trip behind the weight's loads. Every CTA works alone.
+template <int MODE, int COLS>
+struct Skinny {
+    static constexpr int A_BYTES = 16384, B_BYTES = COLS * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int DEPTH = 196608 / STAGE > 10 ? 10 : 196608 / STAGE;
+    static constexpr int BUFS = 512 / COLS > 8 ? 8 : 512 / COLS;
+    static constexpr int TABLE = 32768;  // bytes of scales, MODE FP8
+    static constexpr int SMEM = 1024 + DEPTH * STAGE + TABLE + 256;
+};
+struct SkinnyControl {
+    uint64_t full[10], empty[10], acc_full[8], acc_empty[8];
+    uint32_t tmem;
+    int gave_up;
+};
+static_assert(sizeof(SkinnyControl) <= 512, "control block");
+constexpr int SKINNY_THREADS = 192;
+
+struct SkinnyParams {
+    CUtensorMap a, b;  // weight (128 rows a box) and hidden rows (COLS a box)
+    int V, M, k_blocks, slice, jobs;
+    int* status;
+    const int32_t* targets;
+    float softcap;
+    float2* part;         // [4 CTAs][M]: a warp's maxima and sums over all its tiles
+    float* target_logit;
+    const float* sx;
+    const float* sw;
+    long long sx_stride, sw_stride, out_stride;
+    void* out;
+    int out_bf16;
+};
+
+// COLS columns of this warp's lanes from tensor memory, added (times a scale
+// per column) to sum.
+template <int MODE, int COLS>
+__device__ __forceinline__ void take(uint32_t addr, float (&sum)[COLS], const float* sx, float sw) {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 16) {
+        float v[16];
+        tmem_load16(addr + c, v);
+        tmem_wait_load(v);
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float4 x = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+            if (MODE == FP8) {
+                x = *(const float4*)(sx + c + i);
+                x.x *= sw, x.y *= sw, x.z *= sw, x.w *= sw;
+            }
+            sum[c + i] = fmaf(v[i], x.x, sum[c + i]);
+            sum[c + i + 1] = fmaf(v[i + 1], x.y, sum[c + i + 1]);
+            sum[c + i + 2] = fmaf(v[i + 2], x.z, sum[c + i + 2]);
+            sum[c + i + 3] = fmaf(v[i + 3], x.w, sum[c + i + 3]);
+        }
+    }
+}
+
+template <int MODE, int COLS>
+__global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_constant__ SkinnyParams p) {
+    using S = Skinny<MODE, COLS>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ SkinnyControl ctl;
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* table = (float*)(smem + S::DEPTH * S::STAGE);
+    const uint32_t stage0 = smem_addr(smem);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::DEPTH; ++s) {
+            bar_init(smem_addr(&ctl.full[s]), 1);
+            bar_init(smem_addr(&ctl.empty[s]), 1);
+        }
+        for (int b = 0; b < S::BUFS; ++b) {
+            bar_init(smem_addr(&ctl.acc_full[b]), 1);
+            bar_init(smem_addr(&ctl.acc_empty[b]), 4);
+        }
+        ctl.gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tma_prefetch_map(&p.a);
+        tma_prefetch_map(&p.b);
+    }
+    if (warp == 1) tmem_alloc<false>(smem_addr(&ctl.tmem), 512);
+    if (MODE == FP8) {
+        // the rows' scales, K block by K block: every lane reads the same four at a time
+        for (int i = threadIdx.x; i < p.k_blocks * COLS; i += SKINNY_THREADS) {
+            const int m = i % COLS;
+            table[i] = m < p.M ? p.sx[m * p.sx_stride + i / COLS] : 0.0f;
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = ctl.tmem;
+    volatile int* gave_up = &ctl.gave_up;
+
+    if (warp == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int job = blockIdx.x; ok && job < p.jobs; job += gridDim.x) {
+            for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+                const uint32_t s = it % S::DEPTH;
+                if (!(ok = bar_wait_warp(smem_addr(&ctl.empty[s]), (it / S::DEPTH & 1) ^ 1, gave_up, p.status))) break;
+                if (elected()) {
+                    const uint32_t full = smem_addr(&ctl.full[s]), da = stage0 + s * S::STAGE;
+                    bar_expect(full, S::STAGE);
+                    const int x = kb * (MODE == FP8 ? 128 : 64);
+                    tma_load<false>(da, &p.a, x, job * 128, full);
+                    tma_load<false>(da + S::A_BYTES, &p.b, x, 0, full);
+                }
+                __syncwarp();
+            }
+        }
+        for (uint32_t back = it < S::DEPTH ? it : S::DEPTH; ok && back > 0; --back, ++it)
+            ok = bar_wait_warp(smem_addr(&ctl.empty[it % S::DEPTH]), (it / S::DEPTH & 1) ^ 1, gave_up, p.status);
+    } else if (warp == 1) {
+        uint32_t it = 0, acc = 0;
+        bool ok = true;
+        const uint64_t op0 = operand(stage0, 0);
+        const uint32_t instr = MODE == FP8 ? instr_e4m3(128, COLS) : instr_bf16(128, COLS, false, false);
+        for (int job = blockIdx.x; ok && job < p.jobs; job += gridDim.x) {
+            for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
+                const uint32_t s = it % S::DEPTH, b = acc % S::BUFS;
+                const bool first = kb % p.slice == 0, last = (kb + 1) % p.slice == 0 || kb + 1 == p.k_blocks;
+                if (!(ok = bar_wait_warp(smem_addr(&ctl.full[s]), it / S::DEPTH & 1, gave_up, p.status))) break;
+                if (first && !(ok = bar_wait_warp(smem_addr(&ctl.acc_empty[b]), (acc / S::BUFS & 1) ^ 1, gave_up, p.status)))
+                    break;
+                fence_after();
+                if (elected()) {
+                    const uint64_t oa = op0 + s * (S::STAGE / 16), ob = oa + S::A_BYTES / 16;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        mma<false, MODE == FP8>(tmem + b * COLS, oa + 2 * q, ob + 2 * q, instr, !first || q > 0);
+                    mma_commit<false>(smem_addr(&ctl.empty[s]));
+                    if (last) mma_commit<false>(smem_addr(&ctl.acc_full[b]));
+                }
+                __syncwarp();
+                if (last) ++acc;
+            }
+        }
+    } else {
+        const int quarter = warp % 4;
+        const uint32_t base = tmem + (quarter << 21);
+        const int slices = (p.k_blocks + p.slice - 1) / p.slice;
+        uint32_t acc = 0;
+        bool ok = true;
+        // LSE: each lane's running maximum and sum per row over all its weight rows
+        float mx[MODE == LSE ? COLS : 1], se[MODE == LSE ? COLS : 1];
+#pragma unroll
+        for (int i = 0; i < (MODE == LSE ? COLS : 1); ++i) mx[i] = -3.402823466e38f, se[i] = 0.0f;
+        for (int job = blockIdx.x; ok && job < p.jobs; job += gridDim.x) {
+            const int v0 = job * 128 + quarter * 32, v = v0 + lane;
+            const float* sw = MODE == FP8 ? p.sw + job * p.sw_stride : nullptr;
+            float sum[COLS], w32 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) sum[i] = 0.0f;
+            for (int kb = 0; kb < slices; ++kb, ++acc) {
+                float now = 1.0f;
+                if (MODE == FP8) {
+                    if (kb % 32 == 0) w32 = sw[min(kb + lane, slices - 1)];
+                    now = __shfl_sync(0xffffffffu, w32, kb % 32);
+                }
+                const uint32_t b = acc % S::BUFS;
+                ok = bar_wait_warp(smem_addr(&ctl.acc_full[b]), acc / S::BUFS & 1, gave_up, p.status);
+                if (!ok) break;
+                fence_after();
+                take<MODE, COLS>(base + b * COLS, sum, table + kb * COLS, now);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(smem_addr(&ctl.acc_empty[b]));
+            }
+            if (!ok || v >= p.V) continue;
+            if constexpr (MODE == LSE) {
+#pragma unroll
+                for (int c = 0; c < COLS; c += 16) logits_of(reinterpret_cast<float(&)[16]>(sum[c]), p.softcap);
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) {
+                    if (i < p.M) {
+                        // one exponential: the larger of the two terms is 1
+                        const float l = sum[i], e = exp2_approx(-fabsf(l - mx[i]) * LOG2E);
+                        se[i] = l > mx[i] ? fmaf(se[i], e, 1.0f) : se[i] + e;
+                        mx[i] = fmaxf(mx[i], l);
+                        if (p.targets[i] == v) p.target_logit[i] = l;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) {
+                    if (i < p.M) {
+                        if (p.out_bf16)
+                            ((__nv_bfloat16*)p.out)[i * p.out_stride + v] = __float2bfloat16_rn(sum[i]);
+                        else
+                            ((float*)p.out)[i * p.out_stride + v] = sum[i];
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if constexpr (MODE == LSE) {
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) {
+                if (i < p.M) {
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) {
+                        const float m2 = __shfl_xor_sync(0xffffffffu, mx[i], o), s2 = __shfl_xor_sync(0xffffffffu, se[i], o);
+                        const float top = fmaxf(mx[i], m2);
+                        se[i] = se[i] * exp2_approx((mx[i] - top) * LOG2E) + s2 * exp2_approx((m2 - top) * LOG2E);
+                        mx[i] = top;
+                    }
+                    if (lane == 0) p.part[(long long)(blockIdx.x * 4 + quarter) * p.M + i] = make_float2(mx[i], se[i]);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (*gave_up)
+        for (int i = 0; i < 20; ++i) __nanosleep(1000000);
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        tmem_free<false>(tmem, 512);
+    }
 }
 
 // ---------------------------------------------------------------- joins
@@ -493,10 +752,18 @@ __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* part, cons
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row = blockIdx.x * 32 + lane;
     float mx = -INFINITY, sum = 0.0f;
     if (row < N) {
-        for (int q = warp; q < parts; q += 32) {
-            const float2 x = part[(long long)q * N + row];
-            const float top = fmaxf(mx, x.x), ref = top == -INFINITY ? 0.0f : top;
-            sum = sum * exp2_approx((mx - ref) * LOG2E) + x.y * exp2_approx((x.x - ref) * LOG2E);
+        for (int q = warp; q < parts; q += 32 * 8) {
+            float2 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[i] = q + 32 * i < parts ? part[(long long)(q + 32 * i) * N + row] : make_float2(-INFINITY, 0.0f);
+            float top = mx;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i].x);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            sum *= exp2_approx((mx - ref) * LOG2E);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += x[i].y * exp2_approx((x[i].x - ref) * LOG2E);
             mx = top;
         }
     }
@@ -530,53 +797,206 @@ __global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int sp
 }
 
 // ---------------------------------------------------------------- quantiser
-__device__ __forceinline__ float bf(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-
-// x / s to the nearest e4m3 value, ties to even, as if rounded once: the
-// quotient rounded to 32 bits can only mislead where it lands on the border
-// between two e4m3 values, and there the sign of the exact remainder
-// x - y s (one fma) says on which side of the border the quotient lies.
-__device__ __forceinline__ uint8_t quantize_one(float x, float s) {
-    if (x == 0.0f) return 0;
-    if (s < 0x1p-64f) {  // keeps the remainder out of the subnormals; both products are exact
-        x *= 0x1p80f;
-        s *= 0x1p80f;
-    }
-    float y = __fdiv_rn(x, s);
-    const float ay = fabsf(y);
-    const float step = ay < 0.015625f ? 0.001953125f : __uint_as_float((__float_as_uint(ay) & 0x7f800000u) - (3u << 23));
-    const float h = ay / step;
-    if (h - floorf(h) == 0.5f) {
-        const float r = fmaf(-y, s, x);
-        if (r != 0.0f) y = (r > 0.0f) == (y > 0.0f) ? y * 1.0000002f : y * 0.9999998f;
-    }
-    return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+// The e4m3 code nearest to the exact quotient x / s, ties to even. y is the
+// quotient to a few 2^-24. Only beside a border between two codes can y's own
+// rounding be wrong, and there the sign of the exact remainder x - border s
+// (one fma) says on which side the quotient lies.
+__device__ __forceinline__ uint32_t quantize_border(float x, float s, float y) {
+    const float a = fabsf(y);
+    // the code below: its distance to the next one is 2^-3 of its binade, 2^-9 for the subnormal codes
+    const float step = fmaxf(__uint_as_float((__float_as_uint(a) & 0x7f800000u) - (3u << 23)), 0x1p-9f);
+    const float below = floorf(a * (__uint_as_float((254u << 23) - __float_as_uint(step))));
+    const float border = fmaf(below, step, 0.5f * step), r = fmaf(-border, s, fabsf(x));
+    const bool up = r > 0.0f || (r == 0.0f && ((int)below & 1));
+    return (__nv_cvt_float_to_fp8(below * step, __NV_SATFINITE, __NV_E4M3) + up) | (__float_as_uint(x) >> 24 & 0x80u);
 }
 
-// One block of 128 threads per quantisation block; thread t holds column t.
-__global__ void __launch_bounds__(128) quantize_kernel(const void* x, int bf16, int M, int K, long long x_stride, int rows,
-                                                       uint8_t* q, long long q_stride, float* scale, long long scale_stride) {
-    __shared__ float red[4];
-    const int k = blockIdx.y * FP8_BLOCK + threadIdx.x;
-    const long long m0 = (long long)blockIdx.x * rows, m1 = min(m0 + rows, (long long)M);
-    float mx = 0.0f;
-    bool bad = false;
-    auto at = [&](long long m) { return bf16 ? bf(((const uint16_t*)x)[m * x_stride + k]) : ((const float*)x)[m * x_stride + k]; };
-    if (k < K)
-        for (long long m = m0; m < m1; ++m) {
-            const float v = fabsf(at(m));
-            bad |= !(v < INFINITY);
-            mx = fmaxf(mx, v);
+__device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// A quantisation block's scale, and lo, hi that bracket 1 / scale by 2^-21
+// either way, more than the roundings on the way to x lo and x hi. top: the
+// block's largest magnitude as bits (an infinity or a NaN: NaN for all). A
+// scale below 2^-100 is lifted with its values (exact powers of two).
+struct BlockScale {
+    float s, lo, hi, lifted, lift;
+};
+__device__ __forceinline__ BlockScale block_scale(uint32_t top) {
+    BlockScale b;
+    b.s = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 448.0f) : NAN;
+    b.lift = b.s < 0x1p-100f ? 0x1p120f : 1.0f;
+    b.lifted = b.s * b.lift;
+    const float r = __frcp_rn(b.lifted);
+    b.lo = r * (1.0f - 0x1p-21f);
+    b.hi = r * (1.0f + 0x1p-21f);
+    return b;
+}
+
+// Eight codes of v / b.s. Where x lo and x hi round to one code it is the
+// quotient's; elsewhere (a value beside a border: under 1% of bf16
+// activations, whose few bits often fall on one) the remainder decides. A
+// division per value would cost more than everything else here.
+__device__ __forceinline__ uint2 quantize8(const float (&x)[8], const BlockScale& b) {
+    if (!(b.lifted > 0.0f)) {  // NaN; or 0: a block of zeros, or one whose scale underflowed
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t code = b.s == 0.0f ? (x[i] == 0.0f ? 0u : x[i] < 0.0f ? 0xfeu : 0x7eu) : 0x7fu;
+            w[i / 4] |= code << (8 * (i % 4));
         }
-    if (bad) mx = INFINITY;
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = mx;
+        return make_uint2(w[0], w[1]);
+    }
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i] * b.lift;
+    uint32_t w[2], differ[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w[h] = pack_e4m3(v[4 * h] * b.lo, v[4 * h + 1] * b.lo) | pack_e4m3(v[4 * h + 2] * b.lo, v[4 * h + 3] * b.lo) << 16;
+        differ[h] = w[h] ^ (pack_e4m3(v[4 * h] * b.hi, v[4 * h + 1] * b.hi) |
+                            pack_e4m3(v[4 * h + 2] * b.hi, v[4 * h + 3] * b.hi) << 16);
+    }
+    while (differ[0] | differ[1]) {
+        const int h = differ[0] ? 0 : 1, i = (__ffs(h ? differ[1] : differ[0]) - 1) / 8;
+        const float a = i & 1 ? (h ? v[5] : v[1]) : (h ? v[4] : v[0]), c = i & 1 ? (h ? v[7] : v[3]) : (h ? v[6] : v[2]);
+        const float t = i & 2 ? c : a;
+        const uint32_t mask = 0xffu << (8 * i), code = quantize_border(t, b.lifted, t * b.lo) << (8 * i);
+        if (h) {
+            w[1] = (w[1] & ~mask) | code;
+            differ[1] &= ~mask;
+        } else {
+            w[0] = (w[0] & ~mask) | code;
+            differ[0] &= ~mask;
+        }
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// Eight neighbouring values of a row as they lie in memory; zeros past K.
+template <typename T>
+struct Eight {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const T* row, int k, int K, bool vec) {
+        if (vec && k + 8 <= K) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+                const uint4 u = *(const uint4*)((const unsigned char*)(row + k) + 16 * i);
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k + i < K) {
+                if (sizeof(T) == 2)
+                    w[i / 2] |= (uint32_t)((const uint16_t*)row)[k + i] << (16 * (i % 2));
+                else
+                    w[i % (2 * sizeof(T))] = ((const uint32_t*)row)[k + i];
+            }
+    }
+    // the largest magnitude, as the bits of a float
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * (int)sizeof(T); ++i) {
+            if (sizeof(T) == 2)
+                m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            else
+                m = max(m, w[i] & 0x7fffffffu);
+        }
+        return sizeof(T) == 2 ? max(m & 0xffff0000u, m << 16) : m;
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = __uint_as_float(sizeof(T) == 4 ? w[i % (2 * sizeof(T))] : i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+};
+
+__device__ __forceinline__ void store8(uint8_t* row, int k, int K, bool vec, uint2 w) {
+    if (vec && k + 8 <= K) {
+        *(uint2*)(row + k) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k + i < K) row[k + i] = (uint8_t)((i < 4 ? w.x : w.y) >> (8 * (i % 4)));
+    }
+}
+
+// Blocks of one row: 16 threads a block, eight values a thread, a warp takes
+// 256 columns of QROWS rows with all their loads in flight. Bound by memory:
+// each value is read once and held in registers between the maximum and the
+// quotients.
+constexpr int QROWS = 2;
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, int M, int K, long long x_stride, int x_vec, uint8_t* q,
+                                                            long long q_stride, int q_vec, float* scale,
+                                                            long long scale_stride) {
+    const int lane = threadIdx.x % 32, per_row = (K + 255) / 256;
+    const long long unit = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+    const long long m0 = unit / per_row * QROWS;
+    if (m0 >= M) return;
+    const int k = (int)(unit % per_row) * 256 + lane * 8;
+    Eight<T> e[QROWS];
+#pragma unroll
+    for (int r = 0; r < QROWS; ++r) e[r].load(x + min(m0 + r, (long long)M - 1) * x_stride, k, K, x_vec);
+    uint32_t top[QROWS];
+#pragma unroll
+    for (int r = 0; r < QROWS; ++r) {
+        top[r] = e[r].top();
+#pragma unroll
+        for (int o = 8; o; o >>= 1) top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], o));
+    }
+#pragma unroll
+    for (int r = 0; r < QROWS; ++r) {
+        const BlockScale b = block_scale(top[r]);
+        if (m0 + r < M && k < K) {
+            if (lane % 16 == 0) scale[(m0 + r) * scale_stride + k / FP8_BLOCK] = b.s;
+            float v[8];
+            e[r].values(v);
+            store8(q + (m0 + r) * q_stride, k, K, q_vec, quantize8(v, b));
+        }
+    }
+}
+
+// Blocks of 128 x 128: one CTA each, eight rows' values a thread held in
+// registers between the maximum and the quotients.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_square_kernel(const T* x, int M, int K, long long x_stride, int x_vec, uint8_t* q,
+                                                              long long q_stride, int q_vec, float* scale,
+                                                              long long scale_stride) {
+    __shared__ uint32_t red[8];
+    const int per_row = (K + FP8_BLOCK - 1) / FP8_BLOCK, kb = blockIdx.x % per_row;
+    const long long mb = blockIdx.x / per_row, m0 = mb * FP8_BLOCK + threadIdx.x / 16;
+    const int k = kb * FP8_BLOCK + threadIdx.x % 16 * 8;
+    Eight<T> e[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) e[r].load(x + min(m0 + 16 * r, (long long)M - 1) * x_stride, k, K, x_vec);
+    uint32_t top = 0;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) top = max(top, e[r].top());
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = top;
     __syncthreads();
-    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float s = mx < INFINITY ? __fdiv_rn(mx, 448.0f) : NAN;
-    if (threadIdx.x == 0) scale[blockIdx.x * scale_stride + blockIdx.y] = s;
-    if (k < K)
-        for (long long m = m0; m < m1; ++m) q[m * q_stride + k] = mx < INFINITY ? quantize_one(at(m), s) : 0x7f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, red[i]);
+    const BlockScale b = block_scale(top);
+    if (threadIdx.x == 0) scale[mb * scale_stride + kb] = b.s;
+    if (k >= K) return;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        if (m0 + 16 * r < M) {
+            float v[8];
+            e[r].values(v);
+            store8(q + (m0 + 16 * r) * q_stride, k, K, q_vec, quantize8(v, b));
+        }
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -629,6 +1049,33 @@ cudaError_t launch(const Params& p, int num_sms, cudaStream_t st) {
     return cudaGetLastError();
 }
 
+// The smallest column count that holds the rows, or 0: the pair kernel's.
+int skinny_cols(int rows, int most) {
+    for (int c = 16; c <= most; c *= 2)
+        if (rows <= c) return c;
+    return 0;
+}
+
+template <int MODE, int COLS>
+cudaError_t launch_skinny(SkinnyParams& p, const void* hidden, int esz, long long cols, long long stride, int num_sms,
+                          cudaStream_t st) {
+    using S = Skinny<MODE, COLS>;
+    cudaError_t e = make_map(&p.b, hidden, esz, p.M, cols, stride, COLS);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(skinny_kernel<MODE, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return e;
+    skinny_kernel<MODE, COLS><<<num_sms < p.jobs ? num_sms : p.jobs, SKINNY_THREADS, S::SMEM, st>>>(p);
+    return cudaGetLastError();
+}
+
+constexpr int LSE_SLICE = 16;       // K blocks of 64: sums of 1024 products
+constexpr int LSE_SKINNY_ROWS = 32;
+constexpr int FP8_SKINNY_ROWS = 128;
+
+// Partial sums a row's logits come in.
+long long lse_parts(int N, int V, int num_sms) {
+    return skinny_cols(N, LSE_SKINNY_ROWS) ? 4ll * num_sms : 2 * ceil_div(V, TILE);
+}
+
 // How the gradients are cut: the vocabulary into equal pieces whose dz takes
 // at most DZ_BYTES, and each piece's d_hidden sums into splits along the
 // vocabulary, so that a d_hidden tile is at most half of one pair's share of
@@ -661,8 +1108,8 @@ GradPlan grad_plan(int N, int V, int D, int num_sms) {
 
 using namespace qs;
 
-extern "C" long long qs_head_loss_ws(int N, int V, int, int) {
-    return al(8ll * N * 2 * ceil_div(V, TILE)) + al(4ll * N);
+extern "C" long long qs_head_loss_ws(int N, int V, int, int num_sms) {
+    return al(8ll * N * lse_parts(N, V, num_sms)) + al(4ll * N);
 }
 
 extern "C" long long qs_head_grad_ws(int N, int V, int D, int num_sms) {
@@ -671,25 +1118,50 @@ extern "C" long long qs_head_grad_ws(int N, int V, int D, int num_sms) {
 }
 
 extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream_t st) {
-    Params p = {};
-    cudaError_t e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
-    if (e == cudaSuccess) e = make_map(&p.b, a->weight, 2, a->V, a->D, a->weight_stride, 128);
+    float2* part = (float2*)a->ws;
+    float* target_logit = (float*)(a->ws + al(8ll * a->N * lse_parts(a->N, a->V, a->num_sms)));
+    int parts;
+    cudaError_t e;
+    if (const int cols = skinny_cols(a->N, LSE_SKINNY_ROWS)) {
+        SkinnyParams p = {};
+        e = make_map(&p.a, a->weight, 2, a->V, a->D, a->weight_stride, 128);
+        if (e != cudaSuccess) return e;
+        p.V = a->V;
+        p.M = a->N;
+        p.k_blocks = (int)ceil_div(a->D, 64);
+        p.slice = LSE_SLICE;
+        p.jobs = (int)ceil_div(a->V, 128);
+        p.status = a->status;
+        p.targets = a->targets;
+        p.softcap = a->softcap;
+        p.part = part;
+        p.target_logit = target_logit;
+        parts = 4 * (a->num_sms < p.jobs ? a->num_sms : p.jobs);
+        e = cols == 16 ? launch_skinny<LSE, 16>(p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, st)
+                       : launch_skinny<LSE, 32>(p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, st);
+    } else {
+        Params p = {};
+        e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
+        if (e == cudaSuccess) e = make_map(&p.b, a->weight, 2, a->V, a->D, a->weight_stride, 128);
+        if (e != cudaSuccess) return e;
+        p.m_tiles = (int)ceil_div(a->N, TILE);
+        p.n_tiles = (int)ceil_div(a->V, TILE);
+        p.k_blocks = (int)ceil_div(a->D, 64);
+        p.slice = LSE_SLICE;
+        p.jobs = p.m_tiles * p.n_tiles;
+        p.M = a->N;
+        p.N = a->V;
+        p.status = a->status;
+        p.targets = a->targets;
+        p.softcap = a->softcap;
+        p.part = part;
+        p.target_logit = target_logit;
+        parts = (int)ceil_div(a->V, 128);
+        e = launch<LSE>(p, a->num_sms, st);
+    }
     if (e != cudaSuccess) return e;
-    p.m_tiles = (int)ceil_div(a->N, TILE);
-    p.n_tiles = (int)ceil_div(a->V, TILE);
-    p.k_blocks = (int)ceil_div(a->D, 64);
-    p.jobs = p.m_tiles * p.n_tiles;
-    p.M = a->N;
-    p.N = a->V;
-    p.status = a->status;
-    p.targets = a->targets;
-    p.softcap = a->softcap;
-    p.part = (float2*)a->ws;
-    p.target_logit = (float*)(a->ws + al(8ll * a->N * 2 * p.n_tiles));
-    e = launch<LSE>(p, a->num_sms, st);
-    if (e != cudaSuccess) return e;
-    lse_join_kernel<<<(unsigned)ceil_div(a->N, 32), 1024, 0, st>>>(p.part, p.target_logit, a->targets, a->N, a->V,
-                                                                   (int)ceil_div(a->V, 128), a->loss, a->lse_out);
+    lse_join_kernel<<<(unsigned)ceil_div(a->N, 32), 1024, 0, st>>>(part, target_logit, a->targets, a->N, a->V, parts, a->loss,
+                                                                   a->lse_out);
     *launches = 2;
     return cudaGetLastError();
 }
@@ -711,6 +1183,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.m_tiles = (int)ceil_div(a->N, TILE);
         p.n_tiles = (int)ceil_div(pw, TILE);
         p.k_blocks = (int)ceil_div(a->D, 64);
+        p.slice = INT32_MAX;
         p.jobs = p.m_tiles * p.n_tiles;
         p.M = a->N;
         p.N = pw;
@@ -755,13 +1228,41 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
 }
 
 extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
+    const int cols = skinny_cols(a->M, FP8_SKINNY_ROWS);
+    const long long blocks = ceil_div(a->K, FP8_BLOCK);
+    if (cols && blocks * cols * 4 <= Skinny<FP8, 16>::TABLE) {
+        SkinnyParams p = {};
+        const cudaError_t e = make_map(&p.a, a->w, 1, a->V, a->K, a->w_stride, 128);
+        if (e != cudaSuccess) return e;
+        p.V = a->V;
+        p.M = a->M;
+        p.k_blocks = (int)blocks;
+        p.slice = 1;
+        p.jobs = (int)ceil_div(a->V, 128);
+        p.status = a->status;
+        p.sx = a->sx;
+        p.sw = a->sw;
+        p.sx_stride = a->sx_stride;
+        p.sw_stride = a->sw_stride;
+        p.out = a->out;
+        p.out_stride = a->out_stride;
+        p.out_bf16 = a->out_bf16;
+        switch (cols) {
+            case 16: return launch_skinny<FP8, 16>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
+            case 32: return launch_skinny<FP8, 32>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
+            case 64: return launch_skinny<FP8, 64>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
+            default: return launch_skinny<FP8, 128>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
+        }
+    }
     Params p = {};
     cudaError_t e = make_map(&p.a, a->x, 1, a->M, a->K, a->x_stride, 128);
     if (e == cudaSuccess) e = make_map(&p.b, a->w, 1, a->V, a->K, a->w_stride, 128);
     if (e != cudaSuccess) return e;
     p.m_tiles = (int)ceil_div(a->M, TILE);
     p.n_tiles = (int)ceil_div(a->V, TILE);
-    p.k_blocks = (int)ceil_div(a->K, FP8_BLOCK);
+    p.k_blocks = (int)blocks;
+    p.slice = 1;
+    p.sx_vec = (uintptr_t)a->sx % 16 == 0 && a->sx_stride % 4 == 0;
     p.jobs = p.m_tiles * p.n_tiles;
     p.M = a->M;
     p.N = a->V;
@@ -778,10 +1279,27 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
     return launch<FP8>(p, a->num_sms, st);
 }
 
+template <typename T>
+static cudaError_t quantize(const T* x, int M, int K, long long x_stride, int block_rows, uint8_t* q, long long q_stride,
+                            float* scale, long long scale_stride, cudaStream_t st) {
+    const int x_vec = (uintptr_t)x % 16 == 0 && x_stride * sizeof(T) % 16 == 0;
+    const int q_vec = (uintptr_t)q % 8 == 0 && q_stride % 8 == 0;
+    if (block_rows == 1) {
+        const long long units = ceil_div(M, QROWS) * ceil_div(K, 256);
+        quantize_rows_kernel<T><<<(unsigned)ceil_div(units, 8), 256, 0, st>>>(x, M, K, x_stride, x_vec, q, q_stride, q_vec,
+                                                                              scale, scale_stride);
+    } else {
+        const long long blocks = ceil_div(M, FP8_BLOCK) * ceil_div(K, FP8_BLOCK);
+        quantize_square_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(x, M, K, x_stride, x_vec, q, q_stride, q_vec, scale,
+                                                                    scale_stride);
+    }
+    return cudaGetLastError();
+}
+
 extern "C" cudaError_t qs_quantize_fp8(const void* x, int dtype, int M, int K, long long x_stride, int block_rows,
                                        uint8_t* q, long long q_stride, float* scale, long long scale_stride,
                                        cudaStream_t st) {
-    quantize_kernel<<<dim3((unsigned)ceil_div(M, block_rows), (unsigned)ceil_div(K, FP8_BLOCK)), 128, 0, st>>>(
-        x, dtype == QSAMP_BF16, M, K, x_stride, block_rows, q, q_stride, scale, scale_stride);
-    return cudaGetLastError();
+    if (dtype == QSAMP_BF16)
+        return quantize((const uint16_t*)x, M, K, x_stride, block_rows, q, q_stride, scale, scale_stride, st);
+    return quantize((const float*)x, M, K, x_stride, block_rows, q, q_stride, scale, scale_stride, st);
 }
