@@ -797,80 +797,102 @@ __global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int sp
 }
 
 // ---------------------------------------------------------------- quantiser
-// The e4m3 code nearest to the exact quotient x / s, ties to even. y is the
-// quotient to a few 2^-24. Only beside a border between two codes can y's own
-// rounding be wrong, and there the sign of the exact remainder x - border s
-// (one fma) says on which side the quotient lies.
-__device__ __forceinline__ uint32_t quantize_border(float x, float s, float y) {
-    const float a = fabsf(y);
-    // the code below: its distance to the next one is 2^-3 of its binade, 2^-9 for the subnormal codes
-    const float step = fmaxf(__uint_as_float((__float_as_uint(a) & 0x7f800000u) - (3u << 23)), 0x1p-9f);
-    const float below = floorf(a * (__uint_as_float((254u << 23) - __float_as_uint(step))));
-    const float border = fmaf(below, step, 0.5f * step), r = fmaf(-border, s, fabsf(x));
-    const bool up = r > 0.0f || (r == 0.0f && ((int)below & 1));
-    return (__nv_cvt_float_to_fp8(below * step, __NV_SATFINITE, __NV_E4M3) + up) | (__float_as_uint(x) >> 24 & 0x80u);
-}
-
 __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
 
-// A quantisation block's scale, and lo, hi that bracket 1 / scale by 2^-21
-// either way, more than the roundings on the way to x lo and x hi. top: the
-// block's largest magnitude as bits (an infinity or a NaN: NaN for all). A
-// scale below 2^-100 is lifted with its values (exact powers of two).
+// Two floats in one register pair; one instruction does both.
+struct Two {
+    uint64_t v;
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+    __device__ __forceinline__ explicit Two(uint64_t x) : v(x) {}
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+    return Two(d);
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+    return Two(d);
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return Two(d);
+}
+
+// What quantising by a scale needs: -s, 1 / s (to half a step), (2^19 + 1) / s
+// and 2^38 / s.
+struct Quotient {
+    Two minus_s, inv, inv_split;
+    float inv_big;
+    __device__ __forceinline__ Quotient(float s, float inv)
+        : minus_s(-s), inv(inv), inv_split(inv * 524289.0f), inv_big(inv * 0x1p38f) {}
+};
+
+// Two values whose rounding to e4m3 is that of the exact quotients x / s. The
+// product x inv is off by a few 2^-24, which decides wrongly beside a border
+// between two codes (a few per thousand of bf16 activations lie on one to
+// 2^-24: their few bits over their block's own largest). So it is first cut
+// to h of five bits (Veltkamp's splitting: a sum with 2^19 times itself
+// leaves them): every code and every border is such a number. Which side of h
+// the quotient lies on is the sign of the remainder x - h s, whose fma is
+// exact enough: the remainder is 0 or at least 2^-39 s (29 bits of h s, h from
+// 2^-10 up). That sign, made by a saturated fma, moves h by 1.5 2^-16: enough
+// to leave the largest border (432, steps of 2^-15), and less than the way
+// to a border from the numbers beside the smallest one (2^-10 - 2^-15). A true
+// tie stays on its border and rounds to the even code. All of it runs on
+// the FMA pipe, two values an instruction, and takes no branch.
+__device__ __forceinline__ void round_as_quotients(float& a, float& b, const Quotient& q) {
+    const Two x(a, b), g = mul2(x, q.inv_split), minus(-1.0f);
+    const Two h = add2(g, fma2(g, minus, mul2(x, q.inv)));
+    float ra, rb;
+    fma2(h, q.minus_s, x).get(ra, rb);
+    const Two side = add2(Two(__saturatef(fmaf(ra, q.inv_big, 0.5f)), __saturatef(fmaf(rb, q.inv_big, 0.5f))), Two(-0.5f));
+    fma2(side, Two(3.0f * 0x1p-16f), h).get(a, b);
+}
+
+// A quantisation block's scale and its reciprocal; top: the block's largest
+// magnitude as bits (an infinity or a NaN: NaN for all).
 struct BlockScale {
-    float s, lo, hi, lifted, lift;
+    float s, inv;
 };
 __device__ __forceinline__ BlockScale block_scale(uint32_t top) {
     BlockScale b;
     b.s = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 448.0f) : NAN;
-    b.lift = b.s < 0x1p-100f ? 0x1p120f : 1.0f;
-    b.lifted = b.s * b.lift;
-    const float r = __frcp_rn(b.lifted);
-    b.lo = r * (1.0f - 0x1p-21f);
-    b.hi = r * (1.0f + 0x1p-21f);
+    b.inv = __frcp_rn(b.s);
     return b;
 }
 
-// Eight codes of v / b.s. Where x lo and x hi round to one code it is the
-// quotient's; elsewhere (a value beside a border: under 1% of bf16
-// activations, whose few bits often fall on one) the remainder decides. A
-// division per value would cost more than everything else here.
-__device__ __forceinline__ uint2 quantize8(const float (&x)[8], const BlockScale& b) {
-    if (!(b.lifted > 0.0f)) {  // NaN; or 0: a block of zeros, or one whose scale underflowed
-        uint32_t w[2] = {0, 0};
+__device__ __forceinline__ uint2 quantize8(float (&x)[8], const Quotient& q) {
+    uint32_t w[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t code = b.s == 0.0f ? (x[i] == 0.0f ? 0u : x[i] < 0.0f ? 0xfeu : 0x7eu) : 0x7fu;
-            w[i / 4] |= code << (8 * (i % 4));
-        }
-        return make_uint2(w[0], w[1]);
+    for (int i = 0; i < 8; i += 2) round_as_quotients(x[i], x[i + 1], q);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) w[h] = pack_e4m3(x[4 * h], x[4 * h + 1]) | pack_e4m3(x[4 * h + 2], x[4 * h + 3]) << 16;
+    return make_uint2(w[0], w[1]);
+}
+
+// Scales whose reciprocals or remainders leave the range, and none: NaN.
+constexpr float SMALL_SCALE = 0x1p-60f;
+__device__ __forceinline__ uint2 quantize8_small(float (&x)[8], float s) {
+    if (s > 0.0f) {  // lifted by an exact power of two
+        s *= 0x1p100f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= 0x1p100f;
+        return quantize8(x, Quotient(s, __frcp_rn(s)));
     }
-    float v[8];
+    uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = x[i] * b.lift;
-    uint32_t w[2], differ[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        w[h] = pack_e4m3(v[4 * h] * b.lo, v[4 * h + 1] * b.lo) | pack_e4m3(v[4 * h + 2] * b.lo, v[4 * h + 3] * b.lo) << 16;
-        differ[h] = w[h] ^ (pack_e4m3(v[4 * h] * b.hi, v[4 * h + 1] * b.hi) |
-                            pack_e4m3(v[4 * h + 2] * b.hi, v[4 * h + 3] * b.hi) << 16);
-    }
-    while (differ[0] | differ[1]) {
-        const int h = differ[0] ? 0 : 1, i = (__ffs(h ? differ[1] : differ[0]) - 1) / 8;
-        const float a = i & 1 ? (h ? v[5] : v[1]) : (h ? v[4] : v[0]), c = i & 1 ? (h ? v[7] : v[3]) : (h ? v[6] : v[2]);
-        const float t = i & 2 ? c : a;
-        const uint32_t mask = 0xffu << (8 * i), code = quantize_border(t, b.lifted, t * b.lo) << (8 * i);
-        if (h) {
-            w[1] = (w[1] & ~mask) | code;
-            differ[1] &= ~mask;
-        } else {
-            w[0] = (w[0] & ~mask) | code;
-            differ[0] &= ~mask;
-        }
+    for (int i = 0; i < 8; ++i) {  // 0: a block of zeros, or one whose scale underflowed
+        const uint32_t code = s == 0.0f ? (x[i] == 0.0f ? 0u : x[i] < 0.0f ? 0xfeu : 0x7eu) : 0x7fu;
+        w[i / 4] |= code << (8 * (i % 4));
     }
     return make_uint2(w[0], w[1]);
 }
@@ -880,7 +902,7 @@ template <typename T>
 struct Eight {
     uint32_t w[2 * sizeof(T)];
     __device__ __forceinline__ void load(const T* row, int k, int K, bool vec) {
-        if (vec && k + 8 <= K) {
+        if (vec && k <= K - 8) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
                 const uint4 u = *(const uint4*)((const unsigned char*)(row + k) + 16 * i);
@@ -905,7 +927,7 @@ struct Eight {
 #pragma unroll
         for (int i = 0; i < 2 * (int)sizeof(T); ++i) {
             if (sizeof(T) == 2)
-                m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+                asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
             else
                 m = max(m, w[i] & 0x7fffffffu);
         }
@@ -919,7 +941,7 @@ struct Eight {
 };
 
 __device__ __forceinline__ void store8(uint8_t* row, int k, int K, bool vec, uint2 w) {
-    if (vec && k + 8 <= K) {
+    if (vec && k <= K - 8) {
         *(uint2*)(row + k) = w;
     } else {
 #pragma unroll
@@ -928,75 +950,106 @@ __device__ __forceinline__ void store8(uint8_t* row, int k, int K, bool vec, uin
     }
 }
 
-// Blocks of one row: 16 threads a block, eight values a thread, a warp takes
-// 256 columns of QROWS rows with all their loads in flight. Bound by memory:
-// each value is read once and held in registers between the maximum and the
-// quotients.
-constexpr int QROWS = 2;
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, int M, int K, long long x_stride, int x_vec, uint8_t* q,
-                                                            long long q_stride, int q_vec, float* scale,
-                                                            long long scale_stride) {
-    const int lane = threadIdx.x % 32, per_row = (K + 255) / 256;
-    const long long unit = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-    const long long m0 = unit / per_row * QROWS;
-    if (m0 >= M) return;
-    const int k = (int)(unit % per_row) * 256 + lane * 8;
+// Blocks of one row: 16 threads a block, eight values a thread; a warp takes
+// 256 columns of four rows with all their loads in flight, and eight of its
+// lanes make the eight blocks' scales. Each value is read once and held in
+// registers between the maximum and the quotients. FULL: whole blocks and
+// whole groups of rows on aligned addresses, without checks per value.
+constexpr int QROWS = 4;
+struct QuantArgs {
+    const void* x;
+    uint8_t* q;
+    float* scale;
+    long long x_stride, q_stride, scale_stride;
+    int M, K, x_vec, q_vec;
+};
+template <typename T, bool FULL>
+__device__ __forceinline__ void quantize_rows(const QuantArgs& a, int m0, int k) {
+    const int lane = threadIdx.x % 32;
+    const T* x = (const T*)a.x + m0 * a.x_stride;
     Eight<T> e[QROWS];
 #pragma unroll
-    for (int r = 0; r < QROWS; ++r) e[r].load(x + min(m0 + r, (long long)M - 1) * x_stride, k, K, x_vec);
-    uint32_t top[QROWS];
+    for (int r = 0; r < QROWS; ++r)
+        e[r].load(x + (FULL ? r : min(r, a.M - 1 - m0)) * a.x_stride, k, FULL ? INT32_MAX : a.K, FULL || a.x_vec);
+    uint32_t mine = 0;
 #pragma unroll
     for (int r = 0; r < QROWS; ++r) {
-        top[r] = e[r].top();
+        uint32_t top = e[r].top();
 #pragma unroll
-        for (int o = 8; o; o >>= 1) top[r] = max(top[r], __shfl_xor_sync(0xffffffffu, top[r], o));
+        for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane % QROWS == r) mine = top;
     }
+    const BlockScale b = block_scale(mine);
+    // lane r of a block's sixteen holds row r's scale
+    const int row = lane % 16, kb = k / FP8_BLOCK;
+    if (row < QROWS && m0 + row < a.M && kb * FP8_BLOCK < a.K) a.scale[(m0 + row) * a.scale_stride + kb] = b.s;
+    uint8_t* q = a.q + m0 * a.q_stride;
 #pragma unroll
     for (int r = 0; r < QROWS; ++r) {
-        const BlockScale b = block_scale(top[r]);
-        if (m0 + r < M && k < K) {
-            if (lane % 16 == 0) scale[(m0 + r) * scale_stride + k / FP8_BLOCK] = b.s;
+        const float s = __shfl_sync(0xffffffffu, b.s, (lane & 16) + r), inv = __shfl_sync(0xffffffffu, b.inv, (lane & 16) + r);
+        if (FULL || (m0 + r < a.M && k < a.K)) {
             float v[8];
             e[r].values(v);
-            store8(q + (m0 + r) * q_stride, k, K, q_vec, quantize8(v, b));
+            store8(q + r * a.q_stride, k, FULL ? INT32_MAX : a.K, FULL || a.q_vec,
+                   s >= SMALL_SCALE ? quantize8(v, Quotient(s, inv)) : quantize8_small(v, s));
         }
     }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a, int groups, int log_across) {
+    // a block's eight warps: 2^log_across of them along a row
+    const int warp = threadIdx.x / 32, down = 8 >> log_across;
+    const long long m0 = ((long long)(blockIdx.x / groups) * down + (warp >> log_across)) * QROWS;
+    const int k0 = ((blockIdx.x % groups << log_across) + (warp & ((1 << log_across) - 1))) * 256;
+    if (m0 >= a.M) return;
+    if (a.x_vec && a.q_vec && m0 + QROWS <= a.M && k0 + 256 <= a.K)
+        quantize_rows<T, true>(a, (int)m0, k0 + threadIdx.x % 32 * 8);
+    else
+        quantize_rows<T, false>(a, (int)m0, k0 + threadIdx.x % 32 * 8);
 }
 
 // Blocks of 128 x 128: one CTA each, eight rows' values a thread held in
 // registers between the maximum and the quotients.
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_square_kernel(const T* x, int M, int K, long long x_stride, int x_vec, uint8_t* q,
-                                                              long long q_stride, int q_vec, float* scale,
-                                                              long long scale_stride) {
+template <typename T, bool FULL>
+__device__ __forceinline__ void quantize_square(const QuantArgs& a, int mb, int kb) {
     __shared__ uint32_t red[8];
-    const int per_row = (K + FP8_BLOCK - 1) / FP8_BLOCK, kb = blockIdx.x % per_row;
-    const long long mb = blockIdx.x / per_row, m0 = mb * FP8_BLOCK + threadIdx.x / 16;
-    const int k = kb * FP8_BLOCK + threadIdx.x % 16 * 8;
+    const int m0 = mb * FP8_BLOCK + threadIdx.x / 16, k = kb * FP8_BLOCK + threadIdx.x % 16 * 8;
+    const T* x = (const T*)a.x;
     Eight<T> e[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) e[r].load(x + min(m0 + 16 * r, (long long)M - 1) * x_stride, k, K, x_vec);
+    for (int r = 0; r < 8; ++r)
+        e[r].load(x + (FULL ? m0 + 16 * r : min(m0 + 16 * r, a.M - 1)) * a.x_stride, k, FULL ? INT32_MAX : a.K, FULL || a.x_vec);
     uint32_t top = 0;
 #pragma unroll
     for (int r = 0; r < 8; ++r) top = max(top, e[r].top());
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = __reduce_max_sync(0xffffffffu, top);
     if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = top;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, red[i]);
     const BlockScale b = block_scale(top);
-    if (threadIdx.x == 0) scale[mb * scale_stride + kb] = b.s;
-    if (k >= K) return;
+    if (threadIdx.x == 0) a.scale[mb * a.scale_stride + kb] = b.s;
+    if (!FULL && k >= a.K) return;
+    const Quotient quotient(b.s, b.inv);
+    uint8_t* q = a.q + m0 * a.q_stride;
+    const bool small = !(b.s >= SMALL_SCALE);
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        if (m0 + 16 * r < M) {
+        if (FULL || m0 + 16 * r < a.M) {
             float v[8];
             e[r].values(v);
-            store8(q + (m0 + 16 * r) * q_stride, k, K, q_vec, quantize8(v, b));
+            store8(q + 16 * r * a.q_stride, k, FULL ? INT32_MAX : a.K, FULL || a.q_vec,
+                   small ? quantize8_small(v, b.s) : quantize8(v, quotient));
         }
     }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_square_kernel(const QuantArgs a) {
+    const int per_row = (a.K + FP8_BLOCK - 1) / FP8_BLOCK, kb = blockIdx.x % per_row, mb = blockIdx.x / per_row;
+    if (a.x_vec && a.q_vec && (long long)(mb + 1) * FP8_BLOCK <= a.M && (long long)(kb + 1) * FP8_BLOCK <= a.K)
+        quantize_square<T, true>(a, mb, kb);
+    else
+        quantize_square<T, false>(a, mb, kb);
 }
 
 // ---------------------------------------------------------------- host
@@ -1280,18 +1333,14 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
 }
 
 template <typename T>
-static cudaError_t quantize(const T* x, int M, int K, long long x_stride, int block_rows, uint8_t* q, long long q_stride,
-                            float* scale, long long scale_stride, cudaStream_t st) {
-    const int x_vec = (uintptr_t)x % 16 == 0 && x_stride * sizeof(T) % 16 == 0;
-    const int q_vec = (uintptr_t)q % 8 == 0 && q_stride % 8 == 0;
+static cudaError_t quantize(const QuantArgs& a, int block_rows, cudaStream_t st) {
     if (block_rows == 1) {
-        const long long units = ceil_div(M, QROWS) * ceil_div(K, 256);
-        quantize_rows_kernel<T><<<(unsigned)ceil_div(units, 8), 256, 0, st>>>(x, M, K, x_stride, x_vec, q, q_stride, q_vec,
-                                                                              scale, scale_stride);
+        int log_across = 0;
+        while (log_across < 3 && (256 << log_across) < a.K) ++log_across;
+        const long long groups = ceil_div(a.K, 256 << log_across), down = ceil_div(a.M, QROWS * (8 >> log_across));
+        quantize_rows_kernel<T><<<(unsigned)(groups * down), 256, 0, st>>>(a, (int)groups, log_across);
     } else {
-        const long long blocks = ceil_div(M, FP8_BLOCK) * ceil_div(K, FP8_BLOCK);
-        quantize_square_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(x, M, K, x_stride, x_vec, q, q_stride, q_vec, scale,
-                                                                    scale_stride);
+        quantize_square_kernel<T><<<(unsigned)(ceil_div(a.M, FP8_BLOCK) * ceil_div(a.K, FP8_BLOCK)), 256, 0, st>>>(a);
     }
     return cudaGetLastError();
 }
@@ -1299,7 +1348,9 @@ static cudaError_t quantize(const T* x, int M, int K, long long x_stride, int bl
 extern "C" cudaError_t qs_quantize_fp8(const void* x, int dtype, int M, int K, long long x_stride, int block_rows,
                                        uint8_t* q, long long q_stride, float* scale, long long scale_stride,
                                        cudaStream_t st) {
-    if (dtype == QSAMP_BF16)
-        return quantize((const uint16_t*)x, M, K, x_stride, block_rows, q, q_stride, scale, scale_stride, st);
-    return quantize((const float*)x, M, K, x_stride, block_rows, q, q_stride, scale, scale_stride, st);
+    const int esz = dtype == QSAMP_BF16 ? 2 : 4;
+    QuantArgs a = {x, q, scale, x_stride, q_stride, scale_stride, M, K, 0, 0};
+    a.x_vec = (uintptr_t)x % 16 == 0 && x_stride * esz % 16 == 0;
+    a.q_vec = (uintptr_t)q % 8 == 0 && q_stride % 8 == 0;
+    return esz == 2 ? quantize<uint16_t>(a, block_rows, st) : quantize<float>(a, block_rows, st);
 }

@@ -241,6 +241,49 @@ def test_quantiser_borders(torch, ctx, dtype):
     assert torch.equal(torch.nan_to_num(q.cpu().double(), nan=-1.0), torch.nan_to_num(wq, nan=-1.0))
 
 
+def rounded_e4m3(torch, y):
+    """Doubles to the nearest e4m3 value, ties to even, saturated."""
+    y = y.clamp(-448.0, 448.0)
+    step = torch.ldexp(torch.ones_like(y), torch.frexp(y.abs())[1].sub(1).clamp(min=-6).sub(3))
+    return torch.round(y / step) * step
+
+
+def test_quantiser_every_bf16(torch, ctx):
+    """Every bf16 magnitude below a block's largest, for many largest ones:
+    the codes of the exact quotients. (The quotient of a bf16 by a 32-bit scale
+    is never within 2^-53 of a border without lying on it.)"""
+    allv = torch.arange(1, 0x7F80, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    g = torch.Generator().manual_seed(5)
+    tops = [1.0, 1.5, 448.0, 7.0, 3.5, 1.9921875, 2.0**-60, 2.0**-120, 2.0**100]
+    tops += (1 + torch.randint(0, 128, (24,), generator=g) / 128).tolist()
+    for top in tops:
+        v = allv[(allv.float() <= top) & (allv.float() >= top * 2.0**-22)]
+        v = torch.cat([v, -v])
+        n = -(-v.numel() // 127)
+        x = torch.zeros((n * 127,), dtype=torch.bfloat16)
+        x[:v.numel()] = v
+        x = torch.cat([torch.full((n, 1), top, dtype=torch.bfloat16), x.reshape(n, 127)], dim=1).cuda()
+        q, s = ctx.quantize_fp8(x)
+        assert (s == torch.tensor(top, dtype=torch.float64).div(448).float().item()).all()
+        want = rounded_e4m3(torch, x.double() / s.double())
+        assert torch.equal(q.double(), want), f"largest {top}: {int((q.double() != want).sum())} codes differ"
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+def test_quantiser_large(torch, ctx, rows):
+    """Random values over many binades in blocks of both shapes, both types."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn((1000, 2000), generator=g, device="cuda")
+    x *= torch.exp(4 * torch.randn((1000, 1), generator=g, device="cuda"))
+    for t in (torch.float32, torch.bfloat16):
+        v = x.to(t)
+        q, s = ctx.quantize_fp8(v, block_rows=rows)
+        blocks = torch.nn.functional.max_pool2d(v.double().abs()[None], (rows, 128), ceil_mode=True)[0]
+        assert torch.equal(s, (blocks / torch.full_like(blocks, 448.0)).float())
+        spread = s.double().repeat_interleave(rows, 0)[:1000].repeat_interleave(128, 1)[:, :2000]
+        assert torch.equal(q.double(), rounded_e4m3(torch, v.double() / spread))
+
+
 def test_quantiser_many_rows(torch, ctx):
     """More rows than a grid's second dimension holds."""
     x = torch.full((70000, 16), 2.0, dtype=torch.bfloat16, device="cuda")
