@@ -75,6 +75,19 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
+// Whether the phase is over, without waiting (bar_try may suspend the warp).
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 __device__ __forceinline__ unsigned long long now_ns() {
     unsigned long long t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -110,6 +123,19 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
     return __all_sync(0xffffffffu, bar_wait(bar, parity, gave_up, status));
 }
+
+// Position in a ring of N barriers: the slot and the parity of its phase,
+// stepped rather than divided out (one warp runs these loops, and every
+// dependent instruction of them is latency).
+template <uint32_t N>
+struct Ring {
+    uint32_t slot = 0, parity = 0;
+    __device__ __forceinline__ void step() {
+        const bool wrap = slot == N - 1;
+        slot = wrap ? 0 : slot + 1;
+        parity ^= wrap;
+    }
+};
 
 // ---------------------------------------------------------------- tensor copies
 // Loads the box at (x, y) into this CTA's shared memory and counts its bytes

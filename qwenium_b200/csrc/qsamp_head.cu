@@ -338,21 +338,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
     fence_after();
     const uint32_t tmem = ctl->tmem;
     volatile int* gave_up = &ctl->gave_up;
+    const uint32_t full0 = smem_addr(ctl->full), empty0 = smem_addr(ctl->empty);
+    const uint32_t acc_full0 = smem_addr(ctl->acc_full), acc_empty0 = smem_addr(ctl->acc_empty);
 
     if (warp == 0) {
         // loads: this CTA's half of both operands, counted on the leader's barrier
-        uint32_t it = 0;
+        Ring<STAGES> at;
         bool ok = true;
+        const uint32_t lead_full0 = map_to(full0, 0);
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
             const int m = j.m0 + rank * 128, n = j.n0 + rank * 128;
-            for (int kb = 0; kb < j.k_blocks; ++kb, ++it) {
-                const uint32_t s = it % STAGES;
-                if (!(ok = bar_wait_warp(smem_addr(&ctl->empty[s]), (it / STAGES & 1) ^ 1, gave_up, p.status))) break;
+            for (int kb = 0; kb < j.k_blocks; ++kb, at.step()) {
+                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status))) break;
                 if (elected()) {
-                    const uint32_t full = map_to(smem_addr(&ctl->full[s]), 0);
-                    if (rank == 0) bar_expect(smem_addr(&ctl->full[s]), 2 * STAGE_BYTES);
-                    const uint32_t da = stage0 + s * STAGE_BYTES, db = da + OPERAND_BYTES;
+                    const uint32_t full = lead_full0 + 8 * at.slot;
+                    if (rank == 0) bar_expect(full0 + 8 * at.slot, 2 * STAGE_BYTES);
+                    const uint32_t da = stage0 + at.slot * STAGE_BYTES, db = da + OPERAND_BYTES;
                     if (MODE != GRAD) {
                         const int x = kb * (MODE == FP8 ? 128 : 64);
                         tma_load<true>(da, &p.a, x, m, full);
@@ -374,13 +376,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                 __syncwarp();
             }
         }
-        // the last stages' releases arrive before this CTA may leave
-        for (uint32_t back = it < STAGES ? it : STAGES; ok && back > 0; --back, ++it)
-            ok = bar_wait_warp(smem_addr(&ctl->empty[it % STAGES]), (it / STAGES & 1) ^ 1, gave_up, p.status);
+        // the last stages' releases arrive before this CTA may leave (a stage never used passes at once)
+        for (int back = 0; ok && back < STAGES; ++back, at.step())
+            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status);
     } else if (warp == 1 && rank == 0) {
         // matrix instructions: K blocks of 128 bytes, four instructions each
-        uint32_t it = 0, acc = 0;
-        bool ok = true;
+        // (a barrier takes some 200 cycles to answer: the next ones are asked
+        // while this K block's instructions are issued)
+        Ring<STAGES> at;
+        Ring<2> acc;
+        bool ok = true, full = false, empty = true;
         const uint64_t op0 = operand(stage0, OPERAND_BYTES / 2);
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
@@ -388,31 +393,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
             const uint32_t instr = MODE == FP8 ? instr_e4m3(TILE, TILE) : instr_bf16(TILE, TILE, mn && j.second, mn);
             // along K: 32 bytes of a row, or 16 rows of 128 bytes (operands count 16 bytes)
             const uint32_t step_a = (mn && j.second ? 2048 : 32) / 16, step_b = (mn ? 2048 : 32) / 16;
-            for (int kb = 0; kb < j.k_blocks; ++kb, ++it) {
-                const uint32_t s = it % STAGES;
-                const bool first = kb % p.slice == 0, last = (kb + 1) % p.slice == 0 || kb + 1 == j.k_blocks;
-                if (!(ok = bar_wait_warp(smem_addr(&ctl->full[s]), it / STAGES & 1, gave_up, p.status))) break;
-                if (first && !(ok = bar_wait_warp(smem_addr(&ctl->acc_empty[acc & 1]), (acc / 2 & 1) ^ 1, gave_up, p.status)))
+            int left = 0;  // K blocks to the end of the slice
+            for (int kb = 0; kb < j.k_blocks; ++kb) {
+                const bool first = left == 0;
+                if (first) left = min(p.slice, j.k_blocks - kb);
+                const bool last = --left == 0;
+                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp(full0 + 8 * at.slot, at.parity, gave_up, p.status)))
                     break;
+                if (first && !__all_sync(0xffffffffu, empty) &&
+                    !(ok = bar_wait_warp(acc_empty0 + 8 * acc.slot, acc.parity ^ 1, gave_up, p.status)))
+                    break;
+                const uint32_t slot = at.slot, buf = acc.slot;
+                at.step();
+                full = bar_test(full0 + 8 * at.slot, at.parity);
+                if (last) {
+                    acc.step();
+                    empty = bar_test(acc_empty0 + 8 * acc.slot, acc.parity ^ 1);
+                }
                 fence_after();
                 if (elected()) {
-                    const uint64_t oa = op0 + s * (STAGE_BYTES / 16), ob = oa + OPERAND_BYTES / 16;
-                    const uint32_t d = tmem + (acc & 1) * TILE;
+                    const uint64_t oa = op0 + slot * (STAGE_BYTES / 16), ob = oa + OPERAND_BYTES / 16;
+                    const uint32_t d = tmem + buf * TILE;
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         mma<true, MODE == FP8>(d, oa + q * step_a, ob + q * step_b, instr, !first || q > 0);
-                    mma_commit<true>(smem_addr(&ctl->empty[s]));
-                    if (last) mma_commit<true>(smem_addr(&ctl->acc_full[acc & 1]));
+                    mma_commit<true>(empty0 + 8 * slot);
+                    if (last) mma_commit<true>(acc_full0 + 8 * buf);
                 }
                 __syncwarp();
-                if (last) ++acc;
             }
         }
     } else if (warp >= 2) {
         const int quarter = warp % 4, half = (warp - 2) / 4;
-        uint32_t acc = 0;
+        Ring<2> acc;
         bool ok = true;
-        const uint32_t empty0 = map_to(smem_addr(&ctl->acc_empty[0]), 0), empty1 = map_to(smem_addr(&ctl->acc_empty[1]), 0);
+        const uint32_t lead_empty0 = map_to(acc_empty0, 0);
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
             const int row0 = j.m0 + (int)rank * 128 + quarter * 32, row = row0 + lane;
@@ -426,16 +441,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                     if (target >= p.rows) target = -1;  // DZ: rows holds the vocabulary
                     if (target >= 0) lse = p.lse[row], g = p.grad[row];
                 }
-                ok = bar_wait_warp(smem_addr(&ctl->acc_full[acc & 1]), acc / 2 & 1, gave_up, p.status);
+                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                 if (!ok) break;
                 fence_after();
                 if (row0 < rows)
-                    Epilogue<MODE>::tile(p, j, tmem + (quarter << 21) + (acc & 1) * TILE + half * 128, row, half, live,
+                    Epilogue<MODE>::tile(p, j, tmem + (quarter << 21) + acc.slot * TILE + half * 128, row, half, live,
                                          target, lse, g);
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive_cluster(acc & 1 ? empty1 : empty0);
-                ++acc;
+                if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
+                acc.step();
             } else {
                 // the slices' sums (FP8: a K block each, times its scales) added up in 128 registers
                 float sum[128];
@@ -456,7 +471,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                     sw = p.sw + (col < p.N ? col / 128 : 0) * p.sw_stride;
                     next4 = scales4(sx, 0, slices, p.sx_vec);
                 }
-                for (int kb = 0; kb < slices; ++kb, ++acc) {
+                for (int kb = 0; kb < slices; ++kb, acc.step()) {
                     float now = 1.0f;
                     if (MODE == FP8 && work) {
                         if (kb % 32 == 0) w32 = sw[min(kb + lane, slices - 1)];
@@ -467,25 +482,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                         const float x = kb % 4 < 2 ? (kb % 4 == 0 ? x4.x : x4.y) : (kb % 4 == 2 ? x4.z : x4.w);
                         now = x * __shfl_sync(0xffffffffu, w32, kb % 32);
                     }
-                    ok = bar_wait_warp(smem_addr(&ctl->acc_full[acc & 1]), acc / 2 & 1, gave_up, p.status);
+                    ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                     if (!ok) break;
                     fence_after();
                     if (work) {
 #pragma unroll
                         for (int c = 0; c < 128; c += 32) {
                             float v[32];
-                            tmem_load32(tmem + (quarter << 21) + (acc & 1) * TILE + half * 128 + c, v);
+                            tmem_load32(tmem + (quarter << 21) + acc.slot * TILE + half * 128 + c, v);
                             tmem_wait_load(v);
                             if (c == 96) {
                                 fence_before();
                                 __syncwarp();
-                                if (lane == 0) bar_arrive_cluster(acc & 1 ? empty1 : empty0);
+                                if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
                             }
 #pragma unroll
                             for (int i = 0; i < 32; ++i) sum[c + i] = MODE == FP8 ? fmaf(v[i], now, sum[c + i]) : sum[c + i] + v[i];
                         }
                     } else if (lane == 0) {
-                        bar_arrive_cluster(acc & 1 ? empty1 : empty0);
+                        bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
                     }
                 }
                 if (ok && work) {
@@ -613,16 +628,17 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
     fence_after();
     const uint32_t tmem = ctl.tmem;
     volatile int* gave_up = &ctl.gave_up;
+    const uint32_t full0 = smem_addr(ctl.full), empty0 = smem_addr(ctl.empty);
+    const uint32_t acc_full0 = smem_addr(ctl.acc_full), acc_empty0 = smem_addr(ctl.acc_empty);
 
     if (warp == 0) {
-        uint32_t it = 0;
+        Ring<S::DEPTH> at;
         bool ok = true;
         for (int job = blockIdx.x; ok && job < p.jobs; job += gridDim.x) {
-            for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-                const uint32_t s = it % S::DEPTH;
-                if (!(ok = bar_wait_warp(smem_addr(&ctl.empty[s]), (it / S::DEPTH & 1) ^ 1, gave_up, p.status))) break;
+            for (int kb = 0; kb < p.k_blocks; ++kb, at.step()) {
+                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status))) break;
                 if (elected()) {
-                    const uint32_t full = smem_addr(&ctl.full[s]), da = stage0 + s * S::STAGE;
+                    const uint32_t full = full0 + 8 * at.slot, da = stage0 + at.slot * S::STAGE;
                     bar_expect(full, S::STAGE);
                     const int x = kb * (MODE == FP8 ? 128 : 64);
                     tma_load<false>(da, &p.a, x, job * 128, full);
@@ -631,38 +647,49 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
                 __syncwarp();
             }
         }
-        for (uint32_t back = it < S::DEPTH ? it : S::DEPTH; ok && back > 0; --back, ++it)
-            ok = bar_wait_warp(smem_addr(&ctl.empty[it % S::DEPTH]), (it / S::DEPTH & 1) ^ 1, gave_up, p.status);
+        for (int back = 0; ok && back < S::DEPTH; ++back, at.step())
+            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status);
     } else if (warp == 1) {
-        uint32_t it = 0, acc = 0;
-        bool ok = true;
+        Ring<S::DEPTH> at;
+        Ring<S::BUFS> acc;
+        bool ok = true, full = false, empty = true;
         const uint64_t op0 = operand(stage0, 0);
         const uint32_t instr = MODE == FP8 ? instr_e4m3(128, COLS) : instr_bf16(128, COLS, false, false);
         for (int job = blockIdx.x; ok && job < p.jobs; job += gridDim.x) {
-            for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-                const uint32_t s = it % S::DEPTH, b = acc % S::BUFS;
-                const bool first = kb % p.slice == 0, last = (kb + 1) % p.slice == 0 || kb + 1 == p.k_blocks;
-                if (!(ok = bar_wait_warp(smem_addr(&ctl.full[s]), it / S::DEPTH & 1, gave_up, p.status))) break;
-                if (first && !(ok = bar_wait_warp(smem_addr(&ctl.acc_empty[b]), (acc / S::BUFS & 1) ^ 1, gave_up, p.status)))
+            int left = 0;  // K blocks to the end of the slice
+            for (int kb = 0; kb < p.k_blocks; ++kb) {
+                const bool first = left == 0;
+                if (first) left = min(p.slice, p.k_blocks - kb);
+                const bool last = --left == 0;
+                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp(full0 + 8 * at.slot, at.parity, gave_up, p.status)))
                     break;
+                if (first && !__all_sync(0xffffffffu, empty) &&
+                    !(ok = bar_wait_warp(acc_empty0 + 8 * acc.slot, acc.parity ^ 1, gave_up, p.status)))
+                    break;
+                const uint32_t slot = at.slot, buf = acc.slot;
+                at.step();
+                full = bar_test(full0 + 8 * at.slot, at.parity);
+                if (last) {
+                    acc.step();
+                    empty = bar_test(acc_empty0 + 8 * acc.slot, acc.parity ^ 1);
+                }
                 fence_after();
                 if (elected()) {
-                    const uint64_t oa = op0 + s * (S::STAGE / 16), ob = oa + S::A_BYTES / 16;
+                    const uint64_t oa = op0 + slot * (S::STAGE / 16), ob = oa + S::A_BYTES / 16;
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        mma<false, MODE == FP8>(tmem + b * COLS, oa + 2 * q, ob + 2 * q, instr, !first || q > 0);
-                    mma_commit<false>(smem_addr(&ctl.empty[s]));
-                    if (last) mma_commit<false>(smem_addr(&ctl.acc_full[b]));
+                        mma<false, MODE == FP8>(tmem + buf * COLS, oa + 2 * q, ob + 2 * q, instr, !first || q > 0);
+                    mma_commit<false>(empty0 + 8 * slot);
+                    if (last) mma_commit<false>(acc_full0 + 8 * buf);
                 }
                 __syncwarp();
-                if (last) ++acc;
             }
         }
     } else {
         const int quarter = warp % 4;
         const uint32_t base = tmem + (quarter << 21);
         const int slices = (p.k_blocks + p.slice - 1) / p.slice;
-        uint32_t acc = 0;
+        Ring<S::BUFS> acc;
         bool ok = true;
         // LSE: each lane's running maximum and sum per row over all its weight rows
         float mx[MODE == LSE ? COLS : 1], se[MODE == LSE ? COLS : 1];
@@ -674,20 +701,19 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
             float sum[COLS], w32 = 0.0f;
 #pragma unroll
             for (int i = 0; i < COLS; ++i) sum[i] = 0.0f;
-            for (int kb = 0; kb < slices; ++kb, ++acc) {
+            for (int kb = 0; kb < slices; ++kb, acc.step()) {
                 float now = 1.0f;
                 if (MODE == FP8) {
                     if (kb % 32 == 0) w32 = sw[min(kb + lane, slices - 1)];
                     now = __shfl_sync(0xffffffffu, w32, kb % 32);
                 }
-                const uint32_t b = acc % S::BUFS;
-                ok = bar_wait_warp(smem_addr(&ctl.acc_full[b]), acc / S::BUFS & 1, gave_up, p.status);
+                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                 if (!ok) break;
                 fence_after();
-                take<MODE, COLS>(base + b * COLS, sum, table + kb * COLS, now);
+                take<MODE, COLS>(base + acc.slot * COLS, sum, table + kb * COLS, now);
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(smem_addr(&ctl.acc_empty[b]));
+                if (lane == 0) bar_arrive(acc_empty0 + 8 * acc.slot);
             }
             if (!ok || v >= p.V) continue;
             if constexpr (MODE == LSE) {
