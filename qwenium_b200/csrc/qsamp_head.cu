@@ -31,8 +31,6 @@ constexpr int OPERAND_BYTES = 16384;  // one CTA's half of an operand per stage:
 constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
-constexpr int PATCH_PITCH = 33;       // a warp's 32 x 32 patch for stores to unaligned rows
-constexpr int PATCH_FLOATS = 32 * PATCH_PITCH;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Control {
@@ -40,13 +38,13 @@ struct Control {
     uint32_t tmem;
     int gave_up;
 };
-constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * PATCH_FLOATS * 4 + (int)sizeof(Control);
+constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + (int)sizeof(Control);
 
 enum Mode { LSE, DZ, GRAD, FP8 };
 
 // Rows of the left operand are M, of the right one N; jobs are tiles.
 struct Params {
-    CUtensorMap a, b;    // K contiguous (LSE, DZ, FP8; GRAD: dz for d_hidden)
+    CUtensorMap a, b;    // K contiguous (LSE, DZ; GRAD: dz for d_hidden)
     CUtensorMap a2, b2;  // GRAD: dz and hidden with K in the rows (d_weight); b: weight with K in the rows
     int m_tiles, n_tiles, k_blocks, jobs;
     int slice;           // K blocks summed in tensor memory before the epilogue takes them
@@ -69,13 +67,6 @@ struct Params {
     uint16_t* dw;
     long long dw_stride;
     int wide;            // 32-byte stores reach every row of the output
-    // FP8
-    const float* sx;
-    const float* sw;
-    long long sx_stride, sw_stride, out_stride;
-    void* out;
-    int out_bf16;
-    int sx_vec;          // rows of sx on 16-byte boundaries
 };
 
 struct Job {
@@ -115,6 +106,31 @@ __device__ __forceinline__ Job job_of(const Params& p, int job) {
     j.m0 = m * TILE;
     j.n0 = n * TILE;
     return j;
+}
+
+// ---------------------------------------------------------------- packed fp32
+// Two floats in one register pair; one instruction does both.
+struct Two {
+    uint64_t v;
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+    __device__ __forceinline__ explicit Two(uint64_t x) : v(x) {}
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+    return Two(d);
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+    return Two(d);
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return Two(d);
 }
 
 // ---------------------------------------------------------------- epilogues
@@ -254,64 +270,12 @@ struct Epilogue<GRAD> {
     }
 };
 
-// 32 columns of the 8-bit product's rows. Rows on 32-byte boundaries: each
-// thread stores whole sectors of its own row. Otherwise the warp turns its
-// 32 x 32 patch in shared memory and stores one row after the other.
-__device__ __forceinline__ void store_product(const Params& p, const float* v, int row, int row0, int col, float* patch) {
-    const int lane = threadIdx.x % 32;
-    if (p.wide && col + 32 <= p.N) {
-        if (row >= p.M) return;
-        uint32_t w[8];
-        if (p.out_bf16) {
-            uint16_t* out = (uint16_t*)p.out + row * p.out_stride + col;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[16 * h + 2 * i], v[16 * h + 2 * i + 1]);
-                store32(out + 16 * h, w);
-            }
-        } else {
-            float* out = (float*)p.out + row * p.out_stride + col;
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * h + i]);
-                store32(out + 8 * h, w);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) patch[lane * PATCH_PITCH + i] = v[i];
-    __syncwarp();
-    const int rows = min(32, p.M - row0);
-    if (col + lane < p.N) {
-        for (int r = 0; r < rows; ++r) {
-            const float f = patch[r * PATCH_PITCH + lane];
-            const long long at = (row0 + r) * p.out_stride + col + lane;
-            if (p.out_bf16)
-                ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(f);
-            else
-                ((float*)p.out)[at] = f;
-        }
-    }
-    __syncwarp();
-}
-
-// Scales kb .. kb + 3 of a row; past the end whatever is in reach.
-__device__ __forceinline__ float4 scales4(const float* s, int kb, int n, int vec) {
-    if (kb >= n) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (vec && kb + 4 <= n) return *(const float4*)(s + kb);
-    return make_float4(s[kb], s[min(kb + 1, n - 1)], s[min(kb + 2, n - 1)], s[min(kb + 3, n - 1)]);
-}
-
 // ---------------------------------------------------------------- the kernel
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant__ Params p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* patches = (float*)(smem + STAGES * STAGE_BYTES);
-    Control* ctl = (Control*)(patches + EPI_WARPS * PATCH_FLOATS);
+    Control* ctl = (Control*)(smem + STAGES * STAGE_BYTES);
     const uint32_t stage0 = smem_addr(smem);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cta_rank();
@@ -356,7 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                     if (rank == 0) bar_expect(full0 + 8 * at.slot, 2 * STAGE_BYTES);
                     const uint32_t da = stage0 + at.slot * STAGE_BYTES, db = da + OPERAND_BYTES;
                     if (MODE != GRAD) {
-                        const int x = kb * (MODE == FP8 ? 128 : 64);
+                        const int x = kb * 64;
                         tma_load<true>(da, &p.a, x, m, full);
                         tma_load<true>(db, &p.b, x, n, full);
                     } else {
@@ -390,7 +354,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
             const bool mn = MODE == GRAD;
-            const uint32_t instr = MODE == FP8 ? instr_e4m3(TILE, TILE) : instr_bf16(TILE, TILE, mn && j.second, mn);
+            const uint32_t instr = instr_bf16(TILE, TILE, mn && j.second, mn);
             // along K: 32 bytes of a row, or 16 rows of 128 bytes (operands count 16 bytes)
             const uint32_t step_a = (mn && j.second ? 2048 : 32) / 16, step_b = (mn ? 2048 : 32) / 16;
             int left = 0;  // K blocks to the end of the slice
@@ -416,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                     const uint32_t d = tmem + buf * TILE;
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        mma<true, MODE == FP8>(d, oa + q * step_a, ob + q * step_b, instr, !first || q > 0);
+                        mma<true, false>(d, oa + q * step_a, ob + q * step_b, instr, !first || q > 0);
                     mma_commit<true>(empty0 + 8 * slot);
                     if (last) mma_commit<true>(acc_full0 + 8 * buf);
                 }
@@ -452,36 +416,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                 if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
                 acc.step();
             } else {
-                // the slices' sums (FP8: a K block each, times its scales) added up in 128 registers
+                // the slices' sums added up in 128 registers: tensor memory cuts
+                // its sums rather than rounding them, which over D in the
+                // thousands would show in the loss
                 float sum[128];
 #pragma unroll
                 for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
                 const bool work = row0 < p.M;
-                const int col = j.n0 + half * 128, slices = (j.k_blocks + p.slice - 1) / p.slice;
-                int target = -1;
-                if (MODE == LSE && row < p.M) target = p.targets[row];
-                // FP8: a row's scales come four K blocks at a time, one group
-                // ahead; a column block's are held by the lanes, 32 K blocks at a time
-                const float* sx = nullptr;
-                const float* sw = nullptr;
-                float4 x4 = {}, next4 = {};
-                float w32 = 0.0f;
-                if (MODE == FP8 && work) {
-                    sx = p.sx + (row < p.M ? row : 0) * p.sx_stride;
-                    sw = p.sw + (col < p.N ? col / 128 : 0) * p.sw_stride;
-                    next4 = scales4(sx, 0, slices, p.sx_vec);
-                }
-                for (int kb = 0; kb < slices; ++kb, acc.step()) {
-                    float now = 1.0f;
-                    if (MODE == FP8 && work) {
-                        if (kb % 32 == 0) w32 = sw[min(kb + lane, slices - 1)];
-                        if (kb % 4 == 0) {
-                            x4 = next4;
-                            next4 = scales4(sx, kb + 4, slices, p.sx_vec);
-                        }
-                        const float x = kb % 4 < 2 ? (kb % 4 == 0 ? x4.x : x4.y) : (kb % 4 == 2 ? x4.z : x4.w);
-                        now = x * __shfl_sync(0xffffffffu, w32, kb % 32);
-                    }
+                const int slices = (j.k_blocks + p.slice - 1) / p.slice;
+                const int target = row < p.M ? p.targets[row] : -1;
+                for (int q = 0; q < slices; ++q, acc.step()) {
                     ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                     if (!ok) break;
                     fence_after();
@@ -491,33 +435,312 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                             float v[32];
                             tmem_load32(tmem + (quarter << 21) + acc.slot * TILE + half * 128 + c, v);
                             tmem_wait_load(v);
-                            if (c == 96) {
-                                fence_before();
-                                __syncwarp();
-                                if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
-                            }
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sum[c + i] = MODE == FP8 ? fmaf(v[i], now, sum[c + i]) : sum[c + i] + v[i];
+                            for (int i = 0; i < 32; ++i) sum[c + i] += v[i];
                         }
-                    } else if (lane == 0) {
-                        bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
                     }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
                 }
-                if (ok && work) {
-                    if constexpr (MODE == LSE) {
-                        softmax_sums(p, j, sum, row, half, row < p.M, target);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 128; c += 32)
-                            if (col + c < p.N)
-                                store_product(p, sum + c, row, row0, col + c, patches + (warp - 2) * PATCH_FLOATS);
-                    }
-                }
+                if (ok && work) softmax_sums(p, j, sum, row, half, row < p.M, target);
             }
         }
     }
     __syncwarp();
     // a role gave up: whatever it had in flight lands while this CTA is here
+    if (*gave_up)
+        for (int i = 0; i < 20; ++i) __nanosleep(1000000);
+    fence_before();
+    cluster_sync();
+    if (warp == 1) {
+        fence_after();
+        tmem_free<true>(tmem, 512);
+    }
+    cluster_sync();
+}
+
+// ---------------------------------------------------------------- 8-bit product
+// The block-scaled product of many rows. Scales differ from K block to K
+// block, so each block's sums leave tensor memory after four instructions and
+// are added up in registers: a round trip per 512 tensor cycles, which sets
+// the pace. What shortens it: sixteen epilogue warps of 64 columns each (two
+// loads and 32 packed fmas a block), accumulators handed over in halves of
+// 128 columns, so that one half is read while the other is filled, and
+// scales brought to shared memory by asynchronous copies 16 K blocks ahead
+// (read from global memory they cost 800 cycles a block).
+constexpr int WIDE_EPI = 16;
+constexpr int WIDE_THREADS = 32 * (2 + WIDE_EPI);
+constexpr int CHUNK = 16;   // K blocks of scales copied at once
+constexpr int CHUNK_BUFS = 3;
+constexpr int PATCH_ROWS = 16, PATCH_PITCH = 9;  // a warp's patch for stores to unaligned rows: 8 columns
+struct WideControl {
+    uint64_t full[STAGES], empty[STAGES];
+    uint64_t acc_full[4], acc_empty[4];  // [buffer][half]
+    uint64_t scales_full[CHUNK_BUFS], scales_free[CHUNK_BUFS];
+    uint32_t tmem;
+    int gave_up;
+};
+struct WideScales {
+    float x[CHUNK][128];  // this CTA's rows
+    float w[2][CHUNK];    // the tile's two column blocks
+};
+constexpr int WIDE_SMEM = 1024 + STAGES * STAGE_BYTES + CHUNK_BUFS * (int)sizeof(WideScales) +
+                          WIDE_EPI * PATCH_ROWS * PATCH_PITCH * 4 + (int)sizeof(WideControl);
+static_assert(WIDE_SMEM <= 232448, "shared memory of a CTA");
+
+struct WideParams {
+    CUtensorMap a, b;
+    int m_tiles, n_tiles, k_blocks, jobs, M, V;
+    int* status;
+    const float* sx;
+    const float* sw;
+    long long sx_stride, sw_stride, out_stride;
+    void* out;
+    int out_bf16;
+    int wide;  // 32-byte stores reach every row of out
+};
+
+__device__ __forceinline__ void copy4_async(uint32_t dst, const float* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Copies one chunk of a tile's scales; every epilogue thread takes its part
+// and arrives on `bar` when its copies have landed.
+__device__ __forceinline__ void copy_scales(const WideParams& p, WideScales* to, uint32_t bar, int job, int rank, int chunk,
+                                            int thread) {
+    int m, n;
+    tile_of(job, p.m_tiles, p.n_tiles, m, n);
+    const int k0 = chunk * CHUNK, have = min(CHUNK, p.k_blocks - k0);
+    const int kb = thread % CHUNK;
+    if (kb < have) {
+#pragma unroll
+        for (int i = 0; i < 128 * CHUNK / (32 * WIDE_EPI); ++i) {
+            const int r = thread / CHUNK + i * (32 * WIDE_EPI / CHUNK), row = min(m * TILE + rank * 128 + r, p.M - 1);
+            copy4_async(smem_addr(&to->x[kb][r]), p.sx + row * p.sx_stride + k0 + kb);
+        }
+        if (thread < 2 * CHUNK) {
+            const int block = min(n * 2 + thread / CHUNK, (p.V + 127) / 128 - 1);
+            copy4_async(smem_addr(&to->w[thread / CHUNK][kb]), p.sw + block * p.sw_stride + k0 + kb);
+        }
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// 64 columns of a row. Rows on 32-byte boundaries: each thread stores whole
+// sectors of its own. Otherwise the warp turns patches of 16 rows and 8
+// columns in shared memory, and stores four rows' 8 values at a time.
+__device__ __forceinline__ void store_row64(const WideParams& p, const float (&v)[64], int row, int row0, int col, float* patch) {
+    if (p.wide && col + 64 <= p.V) {
+        if (row >= p.M) return;
+        uint32_t w[8];
+        if (p.out_bf16) {
+            uint16_t* out = (uint16_t*)p.out + row * p.out_stride + col;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[16 * h + 2 * i], v[16 * h + 2 * i + 1]);
+                store32(out + 16 * h, w);
+            }
+        } else {
+            float* out = (float*)p.out + row * p.out_stride + col;
+#pragma unroll
+            for (int h = 0; h < 8; ++h) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * h + i]);
+                store32(out + 8 * h, w);
+            }
+        }
+        return;
+    }
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int c = 0; c < 64; c += 8) {
+        if (col + c >= p.V) break;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            if (lane / PATCH_ROWS == part) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) patch[lane % PATCH_ROWS * PATCH_PITCH + i] = v[c + i];
+            }
+            __syncwarp();
+#pragma unroll
+            for (int r = lane / 8; r < PATCH_ROWS; r += 4) {
+                const int at_row = row0 + part * PATCH_ROWS + r, at_col = col + c + lane % 8;
+                if (at_row < p.M && at_col < p.V) {
+                    const float f = patch[r * PATCH_PITCH + lane % 8];
+                    const long long at = at_row * p.out_stride + at_col;
+                    if (p.out_bf16)
+                        ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(f);
+                    else
+                        ((float*)p.out)[at] = f;
+                }
+            }
+            __syncwarp();
+        }
+    }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wide_kernel(const __grid_constant__ WideParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    WideScales* scales = (WideScales*)(smem + STAGES * STAGE_BYTES);
+    float* patches = (float*)(scales + CHUNK_BUFS);
+    WideControl* ctl = (WideControl*)(patches + WIDE_EPI * PATCH_ROWS * PATCH_PITCH);
+    const uint32_t stage0 = smem_addr(smem);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = cta_rank();
+    const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+    const uint32_t full0 = smem_addr(ctl->full), empty0 = smem_addr(ctl->empty);
+    const uint32_t acc_full0 = smem_addr(ctl->acc_full), acc_empty0 = smem_addr(ctl->acc_empty);
+    const uint32_t scales_full0 = smem_addr(ctl->scales_full), scales_free0 = smem_addr(ctl->scales_free);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            bar_init(full0 + 8 * s, 1);
+            bar_init(empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 4; ++b) {
+            bar_init(acc_full0 + 8 * b, 1);
+            bar_init(acc_empty0 + 8 * b, WIDE_EPI);  // half the epilogue warps of both CTAs
+        }
+        for (int b = 0; b < CHUNK_BUFS; ++b) {
+            bar_init(scales_full0 + 8 * b, 32 * WIDE_EPI);
+            bar_init(scales_free0 + 8 * b, WIDE_EPI);
+        }
+        ctl->gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tma_prefetch_map(&p.a);
+        tma_prefetch_map(&p.b);
+    }
+    if (warp == 1) tmem_alloc<true>(smem_addr(&ctl->tmem), 512);
+    __syncwarp();
+    fence_before();
+    cluster_sync();
+    fence_after();
+    const uint32_t tmem = ctl->tmem;
+    volatile int* gave_up = &ctl->gave_up;
+
+    if (warp == 0) {
+        Ring<STAGES> at;
+        bool ok = true;
+        const uint32_t lead_full0 = map_to(full0, 0);
+        for (int job = pair; ok && job < p.jobs; job += pairs) {
+            int m, n;
+            tile_of(job, p.m_tiles, p.n_tiles, m, n);
+            for (int kb = 0; kb < p.k_blocks; ++kb, at.step()) {
+                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status))) break;
+                if (elected()) {
+                    const uint32_t full = lead_full0 + 8 * at.slot, da = stage0 + at.slot * STAGE_BYTES;
+                    if (rank == 0) bar_expect(full0 + 8 * at.slot, 2 * STAGE_BYTES);
+                    tma_load<true>(da, &p.a, kb * 128, m * TILE + rank * 128, full);
+                    tma_load<true>(da + OPERAND_BYTES, &p.b, kb * 128, n * TILE + rank * 128, full);
+                }
+                __syncwarp();
+            }
+        }
+        for (int back = 0; ok && back < STAGES; ++back, at.step())
+            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status);
+    } else if (warp == 1 && rank == 0) {
+        Ring<STAGES> at;
+        Ring<2> acc;
+        bool ok = true, full = false, empty[2] = {true, true};
+        const uint64_t op0 = operand(stage0, 0);
+        constexpr uint32_t instr = instr_e4m3(TILE, TILE / 2);
+        for (int job = pair; ok && job < p.jobs; job += pairs) {
+            for (int kb = 0; ok && kb < p.k_blocks; ++kb) {
+                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp(full0 + 8 * at.slot, at.parity, gave_up, p.status)))
+                    break;
+                const uint32_t slot = at.slot, buf = acc.slot;
+                at.step();
+                full = bar_test(full0 + 8 * at.slot, at.parity);
+                const uint64_t oa = op0 + slot * (STAGE_BYTES / 16), ob = oa + OPERAND_BYTES / 16;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (!__all_sync(0xffffffffu, empty[h]) &&
+                        !(ok = bar_wait_warp(acc_empty0 + 16 * buf + 8 * h, acc.parity ^ 1, gave_up, p.status)))
+                        break;
+                    fence_after();
+                    if (elected()) {
+                        // 64 weight rows of either CTA: the half's columns are 64 of each column block
+                        const uint64_t obh = ob + h * (64 * 128 / 16);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            mma<true, true>(tmem + buf * TILE + h * (TILE / 2), oa + 2 * q, obh + 2 * q, instr, q > 0);
+                        mma_commit<true>(acc_full0 + 16 * buf + 8 * h);
+                        if (h == 1) mma_commit<true>(empty0 + 8 * slot);
+                    }
+                    __syncwarp();
+                }
+                acc.step();
+                empty[0] = bar_test(acc_empty0 + 16 * acc.slot, acc.parity ^ 1);
+                empty[1] = bar_test(acc_empty0 + 16 * acc.slot + 8, acc.parity ^ 1);
+            }
+        }
+    } else if (warp >= 2) {
+        const int thread = threadIdx.x - 64, e = warp - 2, quarter = warp % 4, half = e / 4 / 2, block = e / 4 % 2;
+        const int chunks = (p.k_blocks + CHUNK - 1) / CHUNK;
+        Ring<2> acc;
+        Ring<CHUNK_BUFS> sc, ahead;  // the chunk in use, and the next to copy
+        bool ok = true;
+        const uint32_t full = acc_full0 + 8 * half, lead_empty = map_to(acc_empty0 + 8 * half, 0);
+        const uint32_t lanes = tmem + (quarter << 21) + half * (TILE / 2) + block * 64;
+        if (pair < p.jobs) {
+            copy_scales(p, scales + ahead.slot, scales_full0 + 8 * ahead.slot, pair, rank, 0, thread);
+            ahead.step();
+        }
+        for (int job = pair; ok && job < p.jobs; job += pairs) {
+            int m, n;
+            tile_of(job, p.m_tiles, p.n_tiles, m, n);
+            const int row0 = m * TILE + (int)rank * 128 + quarter * 32, row = row0 + lane;
+            const int col = n * TILE + block * 128 + half * 64;
+            const bool work = row0 < p.M && col < p.V;
+            float sum[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) sum[i] = 0.0f;
+            for (int c = 0; ok && c < chunks; ++c) {
+                const bool more = c + 1 < chunks;
+                if (more || job + pairs < p.jobs) {
+                    ok = bar_wait_warp(scales_free0 + 8 * ahead.slot, ahead.parity ^ 1, gave_up, p.status);
+                    if (!ok) break;
+                    copy_scales(p, scales + ahead.slot, scales_full0 + 8 * ahead.slot, more ? job : job + pairs, rank,
+                                more ? c + 1 : 0, thread);
+                    ahead.step();
+                }
+                ok = bar_wait_warp(scales_full0 + 8 * sc.slot, sc.parity, gave_up, p.status);
+                if (!ok) break;
+                const float* xs = &scales[sc.slot].x[0][quarter * 32 + lane];
+                const float* ws = scales[sc.slot].w[block];
+                const int have = min(CHUNK, p.k_blocks - c * CHUNK);
+                for (int kb = 0; kb < have; ++kb, acc.step()) {
+                    const float s = xs[kb * 128] * ws[kb];
+                    ok = bar_wait_warp(full + 16 * acc.slot, acc.parity, gave_up, p.status);
+                    if (!ok) break;
+                    fence_after();
+                    if (work) {
+                        const Two s2(s);
+#pragma unroll
+                        for (int q = 0; q < 64; q += 16) {
+                            float v[16];
+                            tmem_load16(lanes + acc.slot * TILE + q, v);
+                            tmem_wait_load(v);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2)
+                                fma2(Two(v[i], v[i + 1]), s2, Two(sum[q + i], sum[q + i + 1])).get(sum[q + i], sum[q + i + 1]);
+                        }
+                    }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive_cluster(lead_empty + 16 * acc.slot);
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(scales_free0 + 8 * sc.slot);
+                sc.step();
+            }
+            if (ok && work) store_row64(p, sum, row, row0, col, patches + e * PATCH_ROWS * PATCH_PITCH);
+        }
+    }
+    __syncwarp();
     if (*gave_up)
         for (int i = 0; i < 20; ++i) __nanosleep(1000000);
     fence_before();
@@ -827,30 +1050,6 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
-}
-
-// Two floats in one register pair; one instruction does both.
-struct Two {
-    uint64_t v;
-    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-    __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
-    __device__ __forceinline__ explicit Two(uint64_t x) : v(x) {}
-    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
-    return Two(d);
-}
-__device__ __forceinline__ Two add2(Two a, Two b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
-    return Two(d);
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return Two(d);
 }
 
 // What quantising by a scale needs: -s, 1 / s (to half a step), (2^19 + 1) / s
@@ -1333,18 +1532,17 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
             default: return launch_skinny<FP8, 128>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
         }
     }
-    Params p = {};
+    WideParams p = {};
     cudaError_t e = make_map(&p.a, a->x, 1, a->M, a->K, a->x_stride, 128);
     if (e == cudaSuccess) e = make_map(&p.b, a->w, 1, a->V, a->K, a->w_stride, 128);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WIDE_SMEM);
     if (e != cudaSuccess) return e;
     p.m_tiles = (int)ceil_div(a->M, TILE);
     p.n_tiles = (int)ceil_div(a->V, TILE);
     p.k_blocks = (int)blocks;
-    p.slice = 1;
-    p.sx_vec = (uintptr_t)a->sx % 16 == 0 && a->sx_stride % 4 == 0;
     p.jobs = p.m_tiles * p.n_tiles;
     p.M = a->M;
-    p.N = a->V;
+    p.V = a->V;
     p.status = a->status;
     p.sx = a->sx;
     p.sw = a->sw;
@@ -1355,7 +1553,9 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
     p.out_bf16 = a->out_bf16;
     const int esz = a->out_bf16 ? 2 : 4;
     p.wide = (uintptr_t)a->out % 32 == 0 && a->out_stride * esz % 32 == 0;
-    return launch<FP8>(p, a->num_sms, st);
+    const int pairs = a->num_sms / 2 < p.jobs ? a->num_sms / 2 : p.jobs;
+    wide_kernel<<<2 * pairs, WIDE_THREADS, WIDE_SMEM, st>>>(p);
+    return cudaGetLastError();
 }
 
 template <typename T>
