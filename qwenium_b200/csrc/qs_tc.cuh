@@ -94,6 +94,13 @@ __device__ __forceinline__ unsigned long long now_ns() {
     return t;
 }
 
+// Launches of one call overlap: the next kernel may start its prologue when
+// every block of this one has begun to leave or has said launch_next, and
+// waits in wait_previous, before its first access to global memory, until this
+// one has ended and its writes are visible.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Longest wait of a role for another; a kernel's own copies and matrix
 // instructions finish in microseconds.
 constexpr unsigned long long WAIT_NS = 2000000000ull;

@@ -302,6 +302,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
     fence_after();
     const uint32_t tmem = ctl->tmem;
     volatile int* gave_up = &ctl->gave_up;
+    launch_next();
+    wait_previous();
     const uint32_t full0 = smem_addr(ctl->full), empty0 = smem_addr(ctl->empty);
     const uint32_t acc_full0 = smem_addr(ctl->acc_full), acc_empty0 = smem_addr(ctl->acc_empty);
 
@@ -851,6 +853,7 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
     fence_after();
     const uint32_t tmem = ctl.tmem;
     volatile int* gave_up = &ctl.gave_up;
+    launch_next();
     const uint32_t full0 = smem_addr(ctl.full), empty0 = smem_addr(ctl.empty);
     const uint32_t acc_full0 = smem_addr(ctl.acc_full), acc_empty0 = smem_addr(ctl.acc_empty);
 
@@ -993,41 +996,54 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------- joins
-// lse of a row from its tiles' maxima and sums; 32 rows per block, the tiles
-// split over the warps.
+// lse of a row from its parts' maxima and sums. A block takes eight rows and
+// 128 parts at a time (four a warp), eight such rounds in flight: the sums of
+// few rows come in up to two thousand parts, and their latency is the kernel.
 __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* part, const float* target_logit, const int32_t* targets,
                                                         int N, int V, int parts, float* loss, float* lse_out) {
-    __shared__ float2 red[32][33];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row = blockIdx.x * 32 + lane;
+    __shared__ float2 red[32][8];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row = blockIdx.x * 8 + lane % 8;
     float mx = -INFINITY, sum = 0.0f;
-    if (row < N) {
-        for (int q = warp; q < parts; q += 32 * 8) {
-            float2 x[8];
+    wait_previous();
+    for (int q = warp * 4 + lane / 8; q < parts; q += 128 * 8) {
+        float2 x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[i] = q + 32 * i < parts ? part[(long long)(q + 32 * i) * N + row] : make_float2(-INFINITY, 0.0f);
-            float top = mx;
+        for (int i = 0; i < 8; ++i)
+            x[i] = row < N && q + 128 * i < parts ? part[(long long)(q + 128 * i) * N + row] : make_float2(-INFINITY, 0.0f);
+        float top = mx;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i].x);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            sum *= exp2_approx((mx - ref) * LOG2E);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum += x[i].y * exp2_approx((x[i].x - ref) * LOG2E);
-            mx = top;
-        }
-    }
-    red[warp][lane] = make_float2(mx, sum);
-    __syncthreads();
-    if (warp == 0 && row < N) {
-        float top = -INFINITY;
-        for (int q = 0; q < 32; ++q) top = fmaxf(top, red[q][lane].x);
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i].x);
         const float ref = top == -INFINITY ? 0.0f : top;
-        sum = 0.0f;
-        for (int q = 0; q < 32; ++q) sum += red[q][lane].y * exp2_approx((red[q][lane].x - ref) * LOG2E);
+        sum *= exp2_approx((mx - ref) * LOG2E);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += x[i].y * exp2_approx((x[i].x - ref) * LOG2E);
+        mx = top;
+    }
+#pragma unroll
+    for (int o = 8; o < 32; o *= 2) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, mx, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+        const float top = fmaxf(mx, m2), ref = top == -INFINITY ? 0.0f : top;
+        sum = sum * exp2_approx((mx - ref) * LOG2E) + s2 * exp2_approx((m2 - ref) * LOG2E);
+        mx = top;
+    }
+    if (lane < 8) red[warp][lane] = make_float2(mx, sum);
+    __syncthreads();
+    if (threadIdx.x >= 256) return;
+    // eight warps: warp w joins row w's 32 partial sums
+    const float2 x = red[lane][warp];
+    mx = x.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    sum = x.y * exp2_approx((x.x - ref) * LOG2E);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int r = blockIdx.x * 8 + warp;
+    if (lane == 0 && r < N) {
         const float lse = ref + logf(sum);
-        const int t = targets[row];
-        lse_out[row] = lse;
-        loss[row] = t < 0 ? 0.0f : t < V ? lse - target_logit[row] : NAN;
+        const int t = targets[r];
+        lse_out[r] = lse;
+        loss[r] = t < 0 ? 0.0f : t < V ? lse - target_logit[r] : NAN;
     }
 }
 
@@ -1036,6 +1052,7 @@ __global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int sp
                                                       long long dh_stride) {
     const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8, n = (long long)N * D;
     if (i >= n) return;
+    wait_previous();
     float v[8] = {};
     for (int s = 0; s < splits; ++s) {
         const float4 x = *(const float4*)(slabs + s * n + i), y = *(const float4*)(slabs + s * n + i + 4);
@@ -1318,11 +1335,29 @@ cudaError_t make_map(CUtensorMap* map, const void* base, int esz, long long rows
                : cudaErrorInvalidValue;
 }
 
+// A launch that may begin before the call's previous kernel has ended (the
+// kernel calls wait_previous).
+template <typename... A, typename... B>
+cudaError_t launch_after(void (*kernel)(A...), long long blocks, int threads, int smem, cudaStream_t st, const B&... args) {
+    cudaLaunchConfig_t c = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.gridDim = dim3((unsigned)blocks);
+    c.blockDim = dim3((unsigned)threads);
+    c.dynamicSmemBytes = (size_t)smem;
+    c.stream = st;
+    c.attrs = at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
 template <int MODE>
-cudaError_t launch(const Params& p, int num_sms, cudaStream_t st) {
+cudaError_t launch(const Params& p, int num_sms, bool first, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(head_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
     if (e != cudaSuccess) return e;
     const int pairs = num_sms / 2 < p.jobs ? num_sms / 2 : p.jobs;
+    if (!first) return launch_after(head_kernel<MODE>, 2 * pairs, THREADS, SMEM_BYTES, st, p);
     head_kernel<MODE><<<2 * pairs, THREADS, SMEM_BYTES, st>>>(p);
     return cudaGetLastError();
 }
@@ -1356,9 +1391,12 @@ long long lse_parts(int N, int V, int num_sms) {
 
 // How the gradients are cut: the vocabulary into equal pieces whose dz takes
 // at most DZ_BYTES, and each piece's d_hidden sums into splits along the
-// vocabulary, so that a d_hidden tile is at most half of one pair's share of
-// the launch (few rows: few tiles with a long sum).
+// vocabulary. Few rows make few d_hidden tiles with a long sum; the splits are
+// the number for which the busiest pair has least to do. Job i runs on pair i
+// mod pairs, d_hidden's first: r pairs have one d_hidden job more, and the
+// d_weight jobs left over go to the pairs from r on.
 constexpr long long DZ_BYTES = 256ll << 20;
+constexpr int MAX_SPLITS = 32;
 struct GradPlan {
     int piece, pieces, splits;
     long long dz_bytes, slab_bytes;
@@ -1370,12 +1408,21 @@ GradPlan grad_plan(int N, int V, int D, int num_sms) {
     g.pieces = (int)ceil_div(V, cap);
     g.piece = (int)(ceil_div(ceil_div(V, g.pieces), TILE) * TILE);
     g.pieces = (int)ceil_div(V, g.piece);
-    const long long dt = ceil_div(D, TILE), mt = ceil_div(N, TILE), kb = ceil_div(g.piece, 64);
-    const long long total = mt * dt * kb + ceil_div(g.piece, TILE) * dt * ceil_div(N, 64);
-    long long share = total / (num_sms / 2) / 2;
-    share = share < 16 ? 16 : share;
-    g.splits = (int)ceil_div(kb, share);
-    g.splits = g.splits > 64 ? 64 : g.splits;
+    const long long dt = ceil_div(D, TILE), tiles = ceil_div(N, TILE) * dt, kb = ceil_div(g.piece, 64), pairs = num_sms / 2;
+    // in K blocks; a tile's epilogue that nothing hides costs about two
+    const long long dw = ceil_div(g.piece, TILE) * dt, dw_cost = ceil_div(N, 64) + 2, dw_each = dw / pairs, dw_left = dw % pairs;
+    long long best = INT64_MAX;
+    g.splits = 1;
+    for (long long s = 1; s <= MAX_SPLITS && s * 8 <= kb; ++s) {
+        const long long cost = ceil_div(kb, s) + 2, each = tiles * s / pairs, r = tiles * s % pairs;
+        long long worst = each * cost + (dw_each + (dw_left > 0)) * dw_cost;
+        const long long more = r ? (each + 1) * cost + (dw_each + (dw_left > pairs - r)) * dw_cost : 0;
+        if (more > worst) worst = more;
+        if (worst < best) {
+            best = worst;
+            g.splits = (int)s;
+        }
+    }
     g.dz_bytes = al(2ll * N * g.piece);
     g.slab_bytes = al(4ll * g.splits * N * D);
     return g;
@@ -1435,13 +1482,12 @@ extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream
         p.part = part;
         p.target_logit = target_logit;
         parts = (int)ceil_div(a->V, 128);
-        e = launch<LSE>(p, a->num_sms, st);
+        e = launch<LSE>(p, a->num_sms, true, st);
     }
     if (e != cudaSuccess) return e;
-    lse_join_kernel<<<(unsigned)ceil_div(a->N, 32), 1024, 0, st>>>(part, target_logit, a->targets, a->N, a->V, parts, a->loss,
-                                                                   a->lse_out);
     *launches = 2;
-    return cudaGetLastError();
+    return launch_after(lse_join_kernel, ceil_div(a->N, 8), 1024, 0, st, (const float2*)part, (const float*)target_logit,
+                        a->targets, a->N, a->V, parts, a->loss, a->lse_out);
 }
 
 extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream_t st) {
@@ -1474,7 +1520,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.dz = dz;
         p.dz_pitch = g.piece;
         p.n0 = p0;
-        e = launch<DZ>(p, a->num_sms, st);
+        e = launch<DZ>(p, a->num_sms, q == 0, st);
         if (e != cudaSuccess) return e;
         e = make_map(&p.a, dz, 2, a->N, pw, g.piece, 128);
         if (e == cudaSuccess) e = make_map(&p.b, a->weight, 2, a->V, a->D, a->weight_stride, 64);
@@ -1495,14 +1541,14 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.dw = a->d_weight;
         p.dw_stride = a->d_weight_stride;
         p.wide = (uintptr_t)a->d_weight % 32 == 0 && a->d_weight_stride % 16 == 0;
-        e = launch<GRAD>(p, a->num_sms, st);
+        e = launch<GRAD>(p, a->num_sms, false, st);
         if (e != cudaSuccess) return e;
         *launches += 2;
     }
     const long long n = (long long)a->N * a->D / 8;
-    dh_join_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(slabs, g.splits, a->N, a->D, a->d_hidden, a->d_hidden_stride);
     *launches += 1;
-    return cudaGetLastError();
+    return launch_after(dh_join_kernel, ceil_div(n, 256), 256, 0, st, (const float*)slabs, g.splits, a->N, a->D, a->d_hidden,
+                        a->d_hidden_stride);
 }
 
 extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {

@@ -606,19 +606,21 @@ class Context:
     def _tensor(self, name, t, dtypes, shape):
         """Checks a CUDA tensor argument: its dtype, its shape (None: any
         size), this context's device, unit stride in the last dimension."""
-        if t.device.type != "cuda" or t.device.index != self.device:
+        if not t.is_cuda or t.get_device() != self.device:
             raise QsampError(1, f"{name}: expected a tensor on cuda:{self.device}, got {t.device}")
         if t.dtype not in dtypes:
             raise QsampError(1, f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
-        if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-            raise QsampError(1, f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
+        got = t.shape
+        if len(got) != len(shape) or any(w is not None and w != g for w, g in zip(shape, got)):
+            raise QsampError(1, f"{name}: expected shape {tuple(shape)}, got {tuple(got)}")
+        if got[-1] > 1 and t.stride(-1) != 1:
             raise QsampError(1, f"{name}: expected unit stride in the last dimension, got {t.stride()}")
 
     @staticmethod
     def _row_stride(t):
         """Elements between rows; a single row's stride is free."""
-        return int(t.stride(0)) if t.shape[0] > 1 else -(-int(t.shape[1]) // 16) * 16
+        rows, cols = t.shape
+        return t.stride(0) if rows > 1 else -(-cols // 16) * 16
 
     def _head(self, hidden, weight, targets, softcap):
         import torch

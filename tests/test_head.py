@@ -38,6 +38,10 @@ def test_tensor_checks():
 
     class OnCuda:
         device = torch.device("cuda", 0)
+        is_cuda = True
+
+        def get_device(self):
+            return 0
 
         def __init__(self, t):
             self.t = t
