@@ -164,6 +164,18 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
             : "memory");
 }
 
+// Stores a box from this CTA's shared memory at (x, y); what lies outside the
+// matrix is left out. The thread that issued the stores waits for them:
+// until their source may be written again, or until they are done.
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+                 "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }

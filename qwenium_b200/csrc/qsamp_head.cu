@@ -38,14 +38,20 @@ struct Control {
     uint32_t tmem;
     int gave_up;
 };
-constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + (int)sizeof(Control);
-
 enum Mode { LSE, DZ, GRAD, FP8 };
+
+// DZ and GRAD: a warp's 32 rows of 64 bf16 outputs on their way out.
+constexpr int OUT_PATCH = 4096;
+__host__ __device__ constexpr int smem_bytes(int mode) {
+    return 1024 + STAGES * STAGE_BYTES + (mode == LSE ? 0 : EPI_WARPS * OUT_PATCH) + (int)sizeof(Control);
+}
+static_assert(smem_bytes(GRAD) <= 232448, "shared memory of a CTA");
 
 // Rows of the left operand are M, of the right one N; jobs are tiles.
 struct Params {
     CUtensorMap a, b;    // K contiguous (LSE, DZ; GRAD: dz for d_hidden)
     CUtensorMap a2, b2;  // GRAD: dz and hidden with K in the rows (d_weight); b: weight with K in the rows
+    CUtensorMap o;       // the bf16 output: DZ: dz, GRAD: the piece's rows of d_weight
     int m_tiles, n_tiles, k_blocks, jobs;
     int slice;           // K blocks summed in tensor memory before the epilogue takes them
     int M, N;            // rows of the left and right operand
@@ -57,16 +63,11 @@ struct Params {
     float* target_logit; // [M]
     const float* lse;
     const float* grad;
-    uint16_t* dz;        // [M][dz_pitch], columns from n0
-    long long dz_pitch;
     int n0;              // DZ, GRAD: first vocabulary column of the piece
     // GRAD: jobs below dh_jobs make d_hidden slabs, the rest d_weight
     int dh_jobs, d_tiles, splits, dh_k_blocks, dw_k_blocks, rows, D;
     float* slabs;        // [splits][rows][D]
     int add;             // slabs hold an earlier piece's sums
-    uint16_t* dw;
-    long long dw_stride;
-    int wide;            // 32-byte stores reach every row of the output
 };
 
 struct Job {
@@ -187,83 +188,97 @@ __device__ __forceinline__ void softmax_sums(const Params& p, const Job& j, floa
     }
 }
 
-// dz = g (exp(l - lse) - [target]) (1 - (l / cap)^2), rounded to bf16: the
-// type of the products it goes into. Rows without a gradient are 0.
+// 64 bf16 columns of the warp's 32 rows, a row a lane: through the warp's patch
+// of shared memory (swizzled in 16-byte pieces as the tensor copy reads it) and
+// out as one box. Stored from the lanes themselves a row's bytes would reach
+// the L1 as 32 lines an instruction, which for short sums is the kernel's
+// time.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, const uint32_t (&w)[32], int x, int y, unsigned char* patch) {
+    const int lane = threadIdx.x % 32;
+    if (lane == 0) tma_store_wait_read();
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        *(uint4*)(patch + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) tma_store(map, x, y, smem_addr(patch));
+}
+
 template <int MODE>
 struct Epilogue;
 
+// dz = g (exp(l - lse) - [target]) (1 - (l / cap)^2); 0 for rows without a
+// gradient.
+__device__ __forceinline__ float dz_of(float l, float lse, float g, float inv_cap, bool hot, bool none) {
+    const float y = l * inv_cap, d = exp2_approx((l - lse) * LOG2E) - (hot ? 1.0f : 0.0f);
+    return none ? 0.0f : d * fmaf(-y, y, 1.0f) * g;
+}
+
+// Rounded to bf16, the type of the products dz goes into.
 template <>
 struct Epilogue<DZ> {
-    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, bool live, int target,
-                                float lse, float g) {
-        const bool none = target < 0;
+    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, int target, float lse, float g,
+                                unsigned char* patch) {
         const float inv = p.softcap > 0.0f ? 1.0f / p.softcap : 0.0f;
         const int c0 = j.n0 + half * 128;
-        uint16_t* out = p.dz + row * p.dz_pitch + c0;
 #pragma unroll 1
-        for (int c = 0; c < 128 && c0 + c < p.N; c += 32) {
-            float v[32];
-            tmem_load32(tmem + c, v);
-            tmem_wait_load(v);
-            logits_of(v, p.softcap);
-            const int at = target - (p.n0 + c0 + c);
-            uint32_t w[16];
+        for (int c = 0; c < 128 && c0 + c < p.N; c += 64) {
+            uint32_t w[32];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                float d[2];
+            for (int q = 0; q < 64; q += 32) {
+                float v[32];
+                tmem_load32(tmem + c + q, v);
+                tmem_wait_load(v);
+                logits_of(v, p.softcap);
+                const int at = target - (p.n0 + c0 + c + q);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const float l = v[i + q], y = l * inv;
-                    d[q] = exp2_approx((l - lse) * LOG2E) - (at == i + q ? 1.0f : 0.0f);
-                    d[q] = none ? 0.0f : d[q] * fmaf(-y, y, 1.0f) * g;
-                }
-                w[i / 2] = pack_bf16(d[0], d[1]);
+                for (int i = 0; i < 32; i += 2)
+                    w[(q + i) / 2] = pack_bf16(dz_of(v[i], lse, g, inv, at == i, target < 0),
+                                               dz_of(v[i + 1], lse, g, inv, at == i + 1, target < 0));
             }
-            if (live) {
-                store32(out + c, reinterpret_cast<const uint32_t(&)[8]>(w[0]));
-                store32(out + c + 16, reinterpret_cast<const uint32_t(&)[8]>(w[8]));
-            }
+            store_box(&p.o, w, c0 + c, row - (int)(threadIdx.x % 32), patch);
         }
     }
 };
 
 template <>
 struct Epilogue<GRAD> {
-    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, bool, int, float, float) {
+    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, int, float, float,
+                                unsigned char* patch) {
         const int c0 = j.n0 + half * 128;
-        const bool live = row < (j.second ? p.N : p.rows);
+        if (j.second) {
+#pragma unroll 1
+            for (int c = 0; c < 128 && c0 + c < p.D; c += 64) {
+                uint32_t w[32];
+#pragma unroll
+                for (int q = 0; q < 64; q += 32) {
+                    float v[32];
+                    tmem_load32(tmem + c + q, v);
+                    tmem_wait_load(v);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) w[(q + i) / 2] = pack_bf16(v[i], v[i + 1]);
+                }
+                store_box(&p.o, w, c0 + c, row - (int)(threadIdx.x % 32), patch);
+            }
+            return;
+        }
 #pragma unroll 1
         for (int c = 0; c < 128 && c0 + c < p.D; c += 32) {
             float v[32];
             tmem_load32(tmem + c, v);
             tmem_wait_load(v);
-            if (!live) continue;
-            const int col = c0 + c;
-            if (!j.second) {
-                float* out = p.slabs + ((long long)j.split * p.rows + row) * p.D + col;
+            if (row < p.rows) {
+                float* out = p.slabs + ((long long)j.split * p.rows + row) * p.D + c0 + c;
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
-                    if (col + i >= p.D) break;
+                    if (c0 + c + i >= p.D) break;
                     if (p.add) {
                         const float4 x = *(const float4*)(out + i), y = *(const float4*)(out + i + 4);
                         v[i] += x.x, v[i + 1] += x.y, v[i + 2] += x.z, v[i + 3] += x.w;
                         v[i + 4] += y.x, v[i + 5] += y.y, v[i + 6] += y.z, v[i + 7] += y.w;
                     }
                     store32(out + i, reinterpret_cast<const uint32_t(&)[8]>(v[i]));
-                }
-            } else {
-                uint32_t w[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-                uint16_t* out = p.dw + (long long)(p.n0 + row) * p.dw_stride + col;
-                if (p.wide && col + 32 <= p.D) {
-                    store32(out, reinterpret_cast<const uint32_t(&)[8]>(w[0]));
-                    store32(out + 16, reinterpret_cast<const uint32_t(&)[8]>(w[8]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (col + 8 * i < p.D)
-                            *(uint4*)(out + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                 }
             }
         }
@@ -275,7 +290,8 @@ template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant__ Params p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    Control* ctl = (Control*)(smem + STAGES * STAGE_BYTES);
+    unsigned char* patches = smem + STAGES * STAGE_BYTES;
+    Control* ctl = (Control*)(smem + smem_bytes(MODE) - 1024 - sizeof(Control));
     const uint32_t stage0 = smem_addr(smem);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cta_rank();
@@ -399,10 +415,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
             const int row0 = j.m0 + (int)rank * 128 + quarter * 32, row = row0 + lane;
             if constexpr (MODE == DZ || MODE == GRAD) {
                 const int rows = MODE == GRAD ? (j.second ? p.N : p.rows) : p.M;
-                const bool live = row < rows;
                 int target = -1;
                 float lse = 0.0f, g = 0.0f;
-                if (MODE == DZ && live) {
+                if (MODE == DZ && row < rows) {
                     target = p.targets[row];
                     if (target >= p.rows) target = -1;  // DZ: rows holds the vocabulary
                     if (target >= 0) lse = p.lse[row], g = p.grad[row];
@@ -411,8 +426,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                 if (!ok) break;
                 fence_after();
                 if (row0 < rows)
-                    Epilogue<MODE>::tile(p, j, tmem + (quarter << 21) + acc.slot * TILE + half * 128, row, half, live,
-                                         target, lse, g);
+                    Epilogue<MODE>::tile(p, j, tmem + (quarter << 21) + acc.slot * TILE + half * 128, row, half, target, lse, g,
+                                         patches + (warp - 2) * OUT_PATCH);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
@@ -448,6 +463,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                 if (ok && work) softmax_sums(p, j, sum, row, half, row < p.M, target);
             }
         }
+        // the last boxes leave shared memory, and arrive, before the CTA does
+        if (MODE != LSE && lane == 0) tma_store_wait();
     }
     __syncwarp();
     // a role gave up: whatever it had in flight lands while this CTA is here
@@ -783,8 +800,13 @@ struct SkinnyParams {
     int* status;
     const int32_t* targets;
     float softcap;
-    float2* part;         // [4 CTAs][M]: a warp's maxima and sums over all its tiles
+    float2* part;         // LSE: [4 CTAs][M]: a warp's maxima and sums over all its tiles
     float* target_logit;
+    const float* lse;     // DZ
+    const float* grad;
+    uint16_t* dz;         // DZ: [M][dz_pitch]: the V vocabulary columns from n0
+    long long dz_pitch;
+    int n0, V_total;
     const float* sx;
     const float* sw;
     long long sx_stride, sw_stride, out_stride;
@@ -822,7 +844,7 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
     extern __shared__ unsigned char smem_raw[];
     __shared__ SkinnyControl ctl;
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* table = (float*)(smem + S::DEPTH * S::STAGE);
+    float* table = (float*)(smem + S::DEPTH * S::STAGE);  // FP8: scales [K block][COLS]; DZ: lse, gradient, target [COLS]
     const uint32_t stage0 = smem_addr(smem);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
@@ -841,6 +863,15 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
         tma_prefetch_map(&p.b);
     }
     if (warp == 1) tmem_alloc<false>(smem_addr(&ctl.tmem), 512);
+    launch_next();
+    wait_previous();
+    if (MODE == DZ && threadIdx.x < COLS) {
+        const int i = threadIdx.x, t = i < p.M ? p.targets[i] : -1;
+        const bool has = t >= 0 && t < p.V_total;
+        table[i] = has ? p.lse[i] : 0.0f;
+        table[COLS + i] = has ? p.grad[i] : 0.0f;
+        ((int*)table)[2 * COLS + i] = has ? t - p.n0 : INT32_MIN;
+    }
     if (MODE == FP8) {
         // the rows' scales, K block by K block: every lane reads the same four at a time
         for (int i = threadIdx.x; i < p.k_blocks * COLS; i += SKINNY_THREADS) {
@@ -853,7 +884,6 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
     fence_after();
     const uint32_t tmem = ctl.tmem;
     volatile int* gave_up = &ctl.gave_up;
-    launch_next();
     const uint32_t full0 = smem_addr(ctl.full), empty0 = smem_addr(ctl.empty);
     const uint32_t acc_full0 = smem_addr(ctl.acc_full), acc_empty0 = smem_addr(ctl.acc_empty);
 
@@ -953,6 +983,18 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
                         se[i] = l > mx[i] ? fmaf(se[i], e, 1.0f) : se[i] + e;
                         mx[i] = fmaxf(mx[i], l);
                         if (p.targets[i] == v) p.target_logit[i] = l;
+                    }
+                }
+            } else if constexpr (MODE == DZ) {
+                const float inv = p.softcap > 0.0f ? 1.0f / p.softcap : 0.0f;
+#pragma unroll
+                for (int c = 0; c < COLS; c += 16) logits_of(reinterpret_cast<float(&)[16]>(sum[c]), p.softcap);
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) {
+                    if (i < p.M) {
+                        const int at = ((const int*)table)[2 * COLS + i];
+                        const float d = dz_of(sum[i], table[i], table[COLS + i], inv, at == v, at == INT32_MIN);
+                        ((__nv_bfloat16*)p.dz)[i * p.dz_pitch + v] = __float2bfloat16_rn(d);
                     }
                 }
             } else {
@@ -1318,7 +1360,7 @@ cudaError_t encoder(EncodeFn* out) {
 }
 
 // A matrix [rows][cols] of 1- or 2-byte elements in boxes of 128 bytes x
-// box_rows; what lies outside reads as 0.
+// box_rows; what lies outside reads as 0 and is not written.
 cudaError_t make_map(CUtensorMap* map, const void* base, int esz, long long rows, long long cols, long long stride,
                      int box_rows) {
     EncodeFn fn;
@@ -1354,11 +1396,12 @@ cudaError_t launch_after(void (*kernel)(A...), long long blocks, int threads, in
 
 template <int MODE>
 cudaError_t launch(const Params& p, int num_sms, bool first, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(head_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    constexpr int smem = smem_bytes(MODE);
+    cudaError_t e = cudaFuncSetAttribute(head_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const int pairs = num_sms / 2 < p.jobs ? num_sms / 2 : p.jobs;
-    if (!first) return launch_after(head_kernel<MODE>, 2 * pairs, THREADS, SMEM_BYTES, st, p);
-    head_kernel<MODE><<<2 * pairs, THREADS, SMEM_BYTES, st>>>(p);
+    if (!first) return launch_after(head_kernel<MODE>, 2 * pairs, THREADS, smem, st, p);
+    head_kernel<MODE><<<2 * pairs, THREADS, smem, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -1370,23 +1413,25 @@ int skinny_cols(int rows, int most) {
 }
 
 template <int MODE, int COLS>
-cudaError_t launch_skinny(SkinnyParams& p, const void* hidden, int esz, long long cols, long long stride, int num_sms,
+cudaError_t launch_skinny(SkinnyParams& p, const void* hidden, int esz, long long cols, long long stride, int num_sms, bool first,
                           cudaStream_t st) {
     using S = Skinny<MODE, COLS>;
     cudaError_t e = make_map(&p.b, hidden, esz, p.M, cols, stride, COLS);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(skinny_kernel<MODE, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return e;
-    skinny_kernel<MODE, COLS><<<num_sms < p.jobs ? num_sms : p.jobs, SKINNY_THREADS, S::SMEM, st>>>(p);
+    const int blocks = num_sms < p.jobs ? num_sms : p.jobs;
+    if (!first) return launch_after(skinny_kernel<MODE, COLS>, blocks, SKINNY_THREADS, S::SMEM, st, p);
+    skinny_kernel<MODE, COLS><<<blocks, SKINNY_THREADS, S::SMEM, st>>>(p);
     return cudaGetLastError();
 }
 
 constexpr int LSE_SLICE = 16;       // K blocks of 64: sums of 1024 products
-constexpr int LSE_SKINNY_ROWS = 32;
+constexpr int HEAD_SKINNY_ROWS = 32;
 constexpr int FP8_SKINNY_ROWS = 128;
 
 // Partial sums a row's logits come in.
 long long lse_parts(int N, int V, int num_sms) {
-    return skinny_cols(N, LSE_SKINNY_ROWS) ? 4ll * num_sms : 2 * ceil_div(V, TILE);
+    return skinny_cols(N, HEAD_SKINNY_ROWS) ? 4ll * num_sms : 2 * ceil_div(V, TILE);
 }
 
 // How the gradients are cut: the vocabulary into equal pieces whose dz takes
@@ -1447,7 +1492,7 @@ extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream
     float* target_logit = (float*)(a->ws + al(8ll * a->N * lse_parts(a->N, a->V, a->num_sms)));
     int parts;
     cudaError_t e;
-    if (const int cols = skinny_cols(a->N, LSE_SKINNY_ROWS)) {
+    if (const int cols = skinny_cols(a->N, HEAD_SKINNY_ROWS)) {
         SkinnyParams p = {};
         e = make_map(&p.a, a->weight, 2, a->V, a->D, a->weight_stride, 128);
         if (e != cudaSuccess) return e;
@@ -1462,8 +1507,8 @@ extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream
         p.part = part;
         p.target_logit = target_logit;
         parts = 4 * (a->num_sms < p.jobs ? a->num_sms : p.jobs);
-        e = cols == 16 ? launch_skinny<LSE, 16>(p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, st)
-                       : launch_skinny<LSE, 32>(p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, st);
+        e = cols == 16 ? launch_skinny<LSE, 16>(p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, true, st)
+                       : launch_skinny<LSE, 32>(p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, true, st);
     } else {
         Params p = {};
         e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
@@ -1497,36 +1542,62 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
     const GradPlan g = grad_plan(a->N, a->V, a->D, a->num_sms);
     uint16_t* dz = (uint16_t*)a->ws;
     float* slabs = (float*)(a->ws + g.dz_bytes);
+    const int cols = skinny_cols(a->N, HEAD_SKINNY_ROWS);
     for (int q = 0; q < g.pieces; ++q) {
         const int p0 = q * g.piece, pw = a->V - p0 < g.piece ? a->V - p0 : g.piece;
+        const uint16_t* weight = a->weight + (long long)p0 * a->weight_stride;
+        cudaError_t e;
         Params p = {};
-        cudaError_t e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
-        if (e == cudaSuccess)
-            e = make_map(&p.b, a->weight + (long long)p0 * a->weight_stride, 2, pw, a->D, a->weight_stride, 128);
-        if (e != cudaSuccess) return e;
         p.m_tiles = (int)ceil_div(a->N, TILE);
         p.n_tiles = (int)ceil_div(pw, TILE);
-        p.k_blocks = (int)ceil_div(a->D, 64);
-        p.slice = INT32_MAX;
-        p.jobs = p.m_tiles * p.n_tiles;
         p.M = a->N;
         p.N = pw;
-        p.rows = a->V;
-        p.status = a->status;
-        p.targets = a->targets;
-        p.softcap = a->softcap;
-        p.lse = a->lse;
-        p.grad = a->grad_loss;
-        p.dz = dz;
-        p.dz_pitch = g.piece;
         p.n0 = p0;
-        e = launch<DZ>(p, a->num_sms, q == 0, st);
+        p.status = a->status;
+        if (cols) {
+            SkinnyParams f = {};
+            e = make_map(&f.a, weight, 2, pw, a->D, a->weight_stride, 128);
+            if (e != cudaSuccess) return e;
+            f.V = pw;
+            f.V_total = a->V;
+            f.n0 = p0;
+            f.M = a->N;
+            f.k_blocks = (int)ceil_div(a->D, 64);
+            f.slice = f.k_blocks;
+            f.jobs = (int)ceil_div(pw, 128);
+            f.status = a->status;
+            f.targets = a->targets;
+            f.softcap = a->softcap;
+            f.lse = a->lse;
+            f.grad = a->grad_loss;
+            f.dz = dz;
+            f.dz_pitch = g.piece;
+            e = cols == 16 ? launch_skinny<DZ, 16>(f, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, q == 0, st)
+                           : launch_skinny<DZ, 32>(f, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, q == 0, st);
+        } else {
+            e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
+            if (e == cudaSuccess) e = make_map(&p.b, weight, 2, pw, a->D, a->weight_stride, 128);
+            if (e == cudaSuccess) e = make_map(&p.o, dz, 2, a->N, g.piece, g.piece, 32);
+            if (e != cudaSuccess) return e;
+            p.k_blocks = (int)ceil_div(a->D, 64);
+            p.slice = INT32_MAX;
+            p.jobs = p.m_tiles * p.n_tiles;
+            p.rows = a->V;
+            p.targets = a->targets;
+            p.softcap = a->softcap;
+            p.lse = a->lse;
+            p.grad = a->grad_loss;
+            e = launch<DZ>(p, a->num_sms, q == 0, st);
+        }
         if (e != cudaSuccess) return e;
         e = make_map(&p.a, dz, 2, a->N, pw, g.piece, 128);
         if (e == cudaSuccess) e = make_map(&p.b, a->weight, 2, a->V, a->D, a->weight_stride, 64);
         if (e == cudaSuccess) e = make_map(&p.a2, dz, 2, a->N, pw, g.piece, 64);
         if (e == cudaSuccess) e = make_map(&p.b2, a->hidden, 2, a->N, a->D, a->hidden_stride, 64);
+        if (e == cudaSuccess)
+            e = make_map(&p.o, a->d_weight + (long long)p0 * a->d_weight_stride, 2, pw, a->D, a->d_weight_stride, 32);
         if (e != cudaSuccess) return e;
+        p.slice = INT32_MAX;
         p.d_tiles = (int)ceil_div(a->D, TILE);
         p.dh_k_blocks = (int)ceil_div(pw, 64);
         // every split has a K block; a short last piece adds to the first slabs
@@ -1538,9 +1609,6 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.D = a->D;
         p.slabs = slabs;
         p.add = q > 0;
-        p.dw = a->d_weight;
-        p.dw_stride = a->d_weight_stride;
-        p.wide = (uintptr_t)a->d_weight % 32 == 0 && a->d_weight_stride % 16 == 0;
         e = launch<GRAD>(p, a->num_sms, false, st);
         if (e != cudaSuccess) return e;
         *launches += 2;
@@ -1572,10 +1640,10 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
         p.out_stride = a->out_stride;
         p.out_bf16 = a->out_bf16;
         switch (cols) {
-            case 16: return launch_skinny<FP8, 16>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
-            case 32: return launch_skinny<FP8, 32>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
-            case 64: return launch_skinny<FP8, 64>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
-            default: return launch_skinny<FP8, 128>(p, a->x, 1, a->K, a->x_stride, a->num_sms, st);
+            case 16: return launch_skinny<FP8, 16>(p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
+            case 32: return launch_skinny<FP8, 32>(p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
+            case 64: return launch_skinny<FP8, 64>(p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
+            default: return launch_skinny<FP8, 128>(p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
         }
     }
     WideParams p = {};
