@@ -13,7 +13,6 @@ sampling.cpp:101,140. ``Context.sample_batch`` is the batched device entry.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from typing import Optional, Sequence
@@ -371,7 +370,8 @@ class Context:
         if rc:
             raise QsampError(rc, f"qsamp_create(device={device})")
         self.h = h
-        self.device = device
+        self.device = int(device)
+        self._device_object = None
 
     def close(self):
         if getattr(self, "h", None):
@@ -594,14 +594,29 @@ class Context:
 
 
     # ------------------------------------------------------------ output head
-    def _on(self, stream):
-        """(raw stream, a context in which torch allocates for that stream):
-        `stream`, or torch's current stream of this context's device."""
+    # A decode step's calls here take a few microseconds of device time, so
+    # what these do on the host is kept short.
+    def _empty(self, stream, shape, dtype):
+        """An uninitialised tensor on this context's device, for use on
+        `stream` (None: torch's current stream), from whose memory it comes."""
         import torch
 
         if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream, contextlib.nullcontext()
-        return int(stream), torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=self.device))
+            return torch.empty(shape, dtype=dtype, device=self._torch_device())
+        with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=self.device)):
+            return torch.empty(shape, dtype=dtype, device=self._torch_device())
+
+    def _torch_device(self):
+        if self._device_object is None:
+            import torch
+
+            self._device_object = torch.device("cuda", self.device)
+        return self._device_object
+
+    def _raw_stream(self, stream):
+        import torch
+
+        return torch.cuda.current_stream(self._torch_device()).cuda_stream if stream is None else int(stream)
 
     def _tensor(self, name, t, dtypes, shape):
         """Checks a CUDA tensor argument: its dtype, its shape (None: any
@@ -615,6 +630,7 @@ class Context:
             raise QsampError(1, f"{name}: expected shape {tuple(shape)}, got {tuple(got)}")
         if got[-1] > 1 and t.stride(-1) != 1:
             raise QsampError(1, f"{name}: expected unit stride in the last dimension, got {t.stride()}")
+        return got
 
     @staticmethod
     def _row_stride(t):
@@ -625,36 +641,32 @@ class Context:
     def _head(self, hidden, weight, targets, softcap):
         import torch
 
-        self._tensor("hidden", hidden, (torch.bfloat16,), (None, None))
-        N, D = (int(x) for x in hidden.shape)
-        self._tensor("weight", weight, (torch.bfloat16,), (None, D))
+        N, D = self._tensor("hidden", hidden, (torch.bfloat16,), (None, None))
+        V, _ = self._tensor("weight", weight, (torch.bfloat16,), (None, D))
         self._tensor("targets", targets, (torch.int32,), (N,))
-        h = _Head(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), N, int(weight.shape[0]), D,
-                  self._row_stride(hidden), self._row_stride(weight), float(softcap))
-        return h
+        return _Head(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), N, V, D, self._row_stride(hidden),
+                     self._row_stride(weight), float(softcap))
 
-    def _workspace(self, h, grad):
+    def _workspace(self, h, grad, stream):
         import torch
 
         n = self.lib.qsamp_head_workspace(self.h, h.N, h.V, h.D, grad)
         if n < 0:
             raise QsampError(1, f"head: expected N >= 0, V >= 1, D >= 1, got {h.N}, {h.V}, {h.D}")
-        return torch.empty(n, dtype=torch.uint8, device=f"cuda:{self.device}")
+        return self._empty(stream, n, torch.uint8), n
 
     def head_loss(self, hidden, weight, targets, softcap: float = 0.0, stream=None):
         """qsamp_head_loss on CUDA tensors: hidden bf16 [N][D], weight bf16
         [V][D], targets int32 [N] (negative: no loss for the row). Returns
-        (loss, lse) float32 [N]; -loss is each target's log-probability."""
+        (loss, lse) float32 [N]; -loss is each target's log-probability.
+        `stream`: a raw stream handle (default: torch's current stream)."""
         import torch
 
         h = self._head(hidden, weight, targets, softcap)
-        raw, alloc = self._on(stream)
-        with alloc:
-            ws = self._workspace(h, 0)
-            out = torch.empty((2, h.N), dtype=torch.float32, device=hidden.device)
-        loss, lse = out[0], out[1]
-        self._check(self.lib.qsamp_head_loss(self.h, ctypes.byref(h), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(),
-                                             ws.numel(), raw), "qsamp_head_loss")
+        ws, n = self._workspace(h, 0, stream)
+        loss, lse = self._empty(stream, (2, h.N), torch.float32).unbind()
+        self._check(self.lib.qsamp_head_loss(self.h, ctypes.byref(h), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), n,
+                                             self._raw_stream(stream)), "qsamp_head_loss")
         return loss, lse
 
     def head_loss_grad(self, hidden, weight, targets, lse, grad_loss, softcap: float = 0.0, d_hidden=None,
@@ -667,19 +679,17 @@ class Context:
         h = self._head(hidden, weight, targets, softcap)
         self._tensor("lse", lse, (torch.float32,), (h.N,))
         self._tensor("grad_loss", grad_loss, (torch.float32,), (h.N,))
-        raw, alloc = self._on(stream)
-        with alloc:
-            ws = self._workspace(h, 1)
-            if d_hidden is None:
-                d_hidden = torch.empty((h.N, h.D), dtype=torch.bfloat16, device=hidden.device)
-            if d_weight is None:
-                d_weight = torch.empty((h.V, h.D), dtype=torch.bfloat16, device=hidden.device)
+        if d_hidden is None:
+            d_hidden = self._empty(stream, (h.N, h.D), torch.bfloat16)
+        if d_weight is None:
+            d_weight = self._empty(stream, (h.V, h.D), torch.bfloat16)
         self._tensor("d_hidden", d_hidden, (torch.bfloat16,), (h.N, h.D))
         self._tensor("d_weight", d_weight, (torch.bfloat16,), (h.V, h.D))
+        ws, n = self._workspace(h, 1, stream)
         self._check(self.lib.qsamp_head_loss_grad(self.h, ctypes.byref(h), lse.data_ptr(), grad_loss.data_ptr(),
-                                                  d_hidden.data_ptr(), self._row_stride(d_hidden),
-                                                  d_weight.data_ptr(), self._row_stride(d_weight), ws.data_ptr(),
-                                                  ws.numel(), raw), "qsamp_head_loss_grad")
+                                                  d_hidden.data_ptr(), self._row_stride(d_hidden), d_weight.data_ptr(),
+                                                  self._row_stride(d_weight), ws.data_ptr(), n,
+                                                  self._raw_stream(stream)), "qsamp_head_loss_grad")
         return d_hidden, d_weight
 
     def quantize_fp8(self, x, block_rows: int = 1, stream=None):
@@ -689,20 +699,16 @@ class Context:
         matmul_fp8 reads them. block_rows: 1 (activations) or 128 (weights)."""
         import torch
 
-        self._tensor("x", x, (torch.float32, torch.bfloat16), (None, None))
+        M, K = self._tensor("x", x, (torch.bfloat16, torch.float32), (None, None))
         if block_rows not in (1, 128):
             raise QsampError(1, f"block_rows: expected 1 or 128, got {block_rows}")
-        M, K = (int(v) for v in x.shape)
-        kb = -(-K // 128)
-        raw, alloc = self._on(stream)
-        with alloc:
-            q = torch.empty((M, -(-K // 16) * 16), dtype=torch.float8_e4m3fn, device=x.device)[:, :K]
-            scale = torch.empty((-(-M // block_rows), kb), dtype=torch.float32, device=x.device)
+        kb, padded = -(-K // 128), -(-K // 16) * 16
+        q = self._empty(stream, (M, padded), torch.float8_e4m3fn)
+        scale = self._empty(stream, (-(-M // block_rows), kb), torch.float32)
         self._check(self.lib.qsamp_quantize_fp8(self.h, x.data_ptr(), QSAMP_BF16 if x.dtype == torch.bfloat16 else QSAMP_F32,
-                                                M, K, self._row_stride(x), int(block_rows), q.data_ptr(),
-                                                self._row_stride(q), scale.data_ptr(), max(kb, 1), raw),
-                    "qsamp_quantize_fp8")
-        return q, scale
+                                                M, K, self._row_stride(x), block_rows, q.data_ptr(), padded,
+                                                scale.data_ptr(), kb, self._raw_stream(stream)), "qsamp_quantize_fp8")
+        return q if K == padded else q[:, :K], scale
 
     def matmul_fp8(self, x, x_scale, w, w_scale, out=None, out_dtype=None, stream=None):
         """qsamp_matmul_fp8 on CUDA tensors: x float8_e4m3fn [M][K] with
@@ -711,24 +717,21 @@ class Context:
         unless `out` or `out_dtype` says float32."""
         import torch
 
-        self._tensor("x", x, (torch.float8_e4m3fn,), (None, None))
-        M, K = (int(v) for v in x.shape)
-        self._tensor("w", w, (torch.float8_e4m3fn,), (None, K))
-        V, kb = int(w.shape[0]), -(-K // 128)
+        M, K = self._tensor("x", x, (torch.float8_e4m3fn,), (None, None))
+        V, _ = self._tensor("w", w, (torch.float8_e4m3fn,), (None, K))
+        kb = -(-K // 128)
         self._tensor("x_scale", x_scale, (torch.float32,), (M, kb))
         self._tensor("w_scale", w_scale, (torch.float32,), (-(-V // 128), kb))
-        raw, alloc = self._on(stream)
         if out is None:
-            with alloc:
-                out = torch.empty((M, V), dtype=out_dtype or torch.bfloat16, device=x.device)
+            out = self._empty(stream, (M, V), out_dtype or torch.bfloat16)
         elif out_dtype is not None and out.dtype != out_dtype:
             raise QsampError(1, f"out_dtype: expected out's {out.dtype}, got {out_dtype}")
-        self._tensor("out", out, (torch.float32, torch.bfloat16), (M, V))
+        self._tensor("out", out, (torch.bfloat16, torch.float32), (M, V))
         p = _Fp8Product(x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), M, V, K,
                         self._row_stride(x), self._row_stride(x_scale), self._row_stride(w), self._row_stride(w_scale),
                         out.data_ptr(), QSAMP_BF16 if out.dtype == torch.bfloat16 else QSAMP_F32,
                         self._row_stride(out))
-        self._check(self.lib.qsamp_matmul_fp8(self.h, ctypes.byref(p), raw), "qsamp_matmul_fp8")
+        self._check(self.lib.qsamp_matmul_fp8(self.h, ctypes.byref(p), self._raw_stream(stream)), "qsamp_matmul_fp8")
         return out
 
 
