@@ -772,7 +772,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
 }
 
 // ---------------------------------------------------------------- few rows
-// A decode step's rows (at most 128; 32 for the cross entropy) against the
+// A decode step's rows (at most 128; 64 for the cross entropy) against the
 // whole head: the weight's bytes bound it. Here the weight's rows are the
 // lanes: a CTA multiplies 128 of them by COLS hidden rows at once, so that
 // the matrix instructions cost COLS columns instead of 256, and tensor memory
@@ -780,6 +780,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
 // epilogue's round trip behind the weight's loads. Every CTA works alone.
 template <int MODE, int COLS>
 struct Skinny {
+    static constexpr int PART = COLS < 32 ? COLS : 32;  // columns of an epilogue warp: four warps for each 32
+    static constexpr int EPI = 4 * (COLS / PART), THREADS = 64 + 32 * EPI;
     static constexpr int A_BYTES = 16384, B_BYTES = COLS * 128, STAGE = A_BYTES + B_BYTES;
     static constexpr int DEPTH = 196608 / STAGE > 10 ? 10 : 196608 / STAGE;
     static constexpr int BUFS = 512 / COLS > 8 ? 8 : 512 / COLS;
@@ -792,7 +794,6 @@ struct SkinnyControl {
     int gave_up;
 };
 static_assert(sizeof(SkinnyControl) <= 512, "control block");
-constexpr int SKINNY_THREADS = 192;
 
 struct SkinnyParams {
     CUtensorMap a, b;  // weight (128 rows a box) and hidden rows (COLS a box)
@@ -839,8 +840,9 @@ __device__ __forceinline__ void take(uint32_t addr, float (&sum)[COLS], const fl
 }
 
 template <int MODE, int COLS>
-__global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_constant__ SkinnyParams p) {
+__global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(const __grid_constant__ SkinnyParams p) {
     using S = Skinny<MODE, COLS>;
+    constexpr int PART = S::PART;
     extern __shared__ unsigned char smem_raw[];
     __shared__ SkinnyControl ctl;
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -855,7 +857,7 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
         }
         for (int b = 0; b < S::BUFS; ++b) {
             bar_init(smem_addr(&ctl.acc_full[b]), 1);
-            bar_init(smem_addr(&ctl.acc_empty[b]), 4);
+            bar_init(smem_addr(&ctl.acc_empty[b]), S::EPI);
         }
         ctl.gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -874,7 +876,7 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
     }
     if (MODE == FP8) {
         // the rows' scales, K block by K block: every lane reads the same four at a time
-        for (int i = threadIdx.x; i < p.k_blocks * COLS; i += SKINNY_THREADS) {
+        for (int i = threadIdx.x; i < p.k_blocks * COLS; i += S::THREADS) {
             const int m = i % COLS;
             table[i] = m < p.M ? p.sx[m * p.sx_stride + i / COLS] : 0.0f;
         }
@@ -942,21 +944,21 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
             }
         }
     } else {
-        const int quarter = warp % 4;
-        const uint32_t base = tmem + (quarter << 21);
+        const int quarter = warp % 4, c0 = (warp - 2) / 4 * PART, mine = p.M - c0;  // rows from c0
+        const uint32_t base = tmem + (quarter << 21) + c0;
         const int slices = (p.k_blocks + p.slice - 1) / p.slice;
         Ring<S::BUFS> acc;
         bool ok = true;
         // LSE: each lane's running maximum and sum per row over all its weight rows
-        float mx[MODE == LSE ? COLS : 1], se[MODE == LSE ? COLS : 1];
+        float mx[MODE == LSE ? PART : 1], se[MODE == LSE ? PART : 1];
 #pragma unroll
-        for (int i = 0; i < (MODE == LSE ? COLS : 1); ++i) mx[i] = -3.402823466e38f, se[i] = 0.0f;
+        for (int i = 0; i < (MODE == LSE ? PART : 1); ++i) mx[i] = -3.402823466e38f, se[i] = 0.0f;
         for (int job = blockIdx.x; ok && job < p.jobs; job += gridDim.x) {
             const int v0 = job * 128 + quarter * 32, v = v0 + lane;
             const float* sw = MODE == FP8 ? p.sw + job * p.sw_stride : nullptr;
-            float sum[COLS], w32 = 0.0f;
+            float sum[PART], w32 = 0.0f;  // FP8: the weight block's scales, 32 K blocks in the lanes
 #pragma unroll
-            for (int i = 0; i < COLS; ++i) sum[i] = 0.0f;
+            for (int i = 0; i < PART; ++i) sum[i] = 0.0f;
             for (int kb = 0; kb < slices; ++kb, acc.step()) {
                 float now = 1.0f;
                 if (MODE == FP8) {
@@ -966,7 +968,7 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
                 ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                 if (!ok) break;
                 fence_after();
-                take<MODE, COLS>(base + acc.slot * COLS, sum, table + kb * COLS, now);
+                if (mine > 0) take<MODE, PART>(base + acc.slot * COLS, sum, table + kb * COLS + c0, now);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(acc_empty0 + 8 * acc.slot);
@@ -974,37 +976,38 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
             if (!ok || v >= p.V) continue;
             if constexpr (MODE == LSE) {
 #pragma unroll
-                for (int c = 0; c < COLS; c += 16) logits_of(reinterpret_cast<float(&)[16]>(sum[c]), p.softcap);
+                for (int c = 0; c < PART; c += 16) logits_of(reinterpret_cast<float(&)[16]>(sum[c]), p.softcap);
 #pragma unroll
-                for (int i = 0; i < COLS; ++i) {
-                    if (i < p.M) {
+                for (int i = 0; i < PART; ++i) {
+                    if (i < mine) {
                         // one exponential: the larger of the two terms is 1
                         const float l = sum[i], e = exp2_approx(-fabsf(l - mx[i]) * LOG2E);
                         se[i] = l > mx[i] ? fmaf(se[i], e, 1.0f) : se[i] + e;
                         mx[i] = fmaxf(mx[i], l);
-                        if (p.targets[i] == v) p.target_logit[i] = l;
+                        if (p.targets[c0 + i] == v) p.target_logit[c0 + i] = l;
                     }
                 }
             } else if constexpr (MODE == DZ) {
                 const float inv = p.softcap > 0.0f ? 1.0f / p.softcap : 0.0f;
 #pragma unroll
-                for (int c = 0; c < COLS; c += 16) logits_of(reinterpret_cast<float(&)[16]>(sum[c]), p.softcap);
+                for (int c = 0; c < PART; c += 16) logits_of(reinterpret_cast<float(&)[16]>(sum[c]), p.softcap);
 #pragma unroll
-                for (int i = 0; i < COLS; ++i) {
-                    if (i < p.M) {
-                        const int at = ((const int*)table)[2 * COLS + i];
-                        const float d = dz_of(sum[i], table[i], table[COLS + i], inv, at == v, at == INT32_MIN);
-                        ((__nv_bfloat16*)p.dz)[i * p.dz_pitch + v] = __float2bfloat16_rn(d);
+                for (int i = 0; i < PART; ++i) {
+                    if (i < mine) {
+                        const int at = ((const int*)table)[2 * COLS + c0 + i];
+                        const float d = dz_of(sum[i], table[c0 + i], table[COLS + c0 + i], inv, at == v, at == INT32_MIN);
+                        ((__nv_bfloat16*)p.dz)[(c0 + i) * p.dz_pitch + v] = __float2bfloat16_rn(d);
                     }
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < COLS; ++i) {
-                    if (i < p.M) {
+                for (int i = 0; i < PART; ++i) {
+                    if (i < mine) {
+                        const long long at = (c0 + i) * p.out_stride + v;
                         if (p.out_bf16)
-                            ((__nv_bfloat16*)p.out)[i * p.out_stride + v] = __float2bfloat16_rn(sum[i]);
+                            ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(sum[i]);
                         else
-                            ((float*)p.out)[i * p.out_stride + v] = sum[i];
+                            ((float*)p.out)[at] = sum[i];
                     }
                 }
             }
@@ -1012,8 +1015,8 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
         __syncwarp();
         if constexpr (MODE == LSE) {
 #pragma unroll
-            for (int i = 0; i < COLS; ++i) {
-                if (i < p.M) {
+            for (int i = 0; i < PART; ++i) {
+                if (i < mine) {
 #pragma unroll
                     for (int o = 16; o; o >>= 1) {
                         const float m2 = __shfl_xor_sync(0xffffffffu, mx[i], o), s2 = __shfl_xor_sync(0xffffffffu, se[i], o);
@@ -1021,7 +1024,7 @@ __global__ void __launch_bounds__(SKINNY_THREADS, 1) skinny_kernel(const __grid_
                         se[i] = se[i] * exp2_approx((mx[i] - top) * LOG2E) + s2 * exp2_approx((m2 - top) * LOG2E);
                         mx[i] = top;
                     }
-                    if (lane == 0) p.part[(long long)(blockIdx.x * 4 + quarter) * p.M + i] = make_float2(mx[i], se[i]);
+                    if (lane == 0) p.part[(long long)(blockIdx.x * 4 + quarter) * p.M + c0 + i] = make_float2(mx[i], se[i]);
                 }
             }
         }
@@ -1407,9 +1410,10 @@ cudaError_t launch(const Params& p, int num_sms, bool first, cudaStream_t st) {
 
 // The smallest column count that holds the rows, or 0: the pair kernel's.
 int skinny_cols(int rows, int most) {
-    for (int c = 16; c <= most; c *= 2)
+    if (rows > most) return 0;
+    for (int c = 16; c < 128; c *= 2)
         if (rows <= c) return c;
-    return 0;
+    return 128;
 }
 
 template <int MODE, int COLS>
@@ -1420,13 +1424,27 @@ cudaError_t launch_skinny(SkinnyParams& p, const void* hidden, int esz, long lon
     if (e == cudaSuccess) e = cudaFuncSetAttribute(skinny_kernel<MODE, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return e;
     const int blocks = num_sms < p.jobs ? num_sms : p.jobs;
-    if (!first) return launch_after(skinny_kernel<MODE, COLS>, blocks, SKINNY_THREADS, S::SMEM, st, p);
-    skinny_kernel<MODE, COLS><<<blocks, SKINNY_THREADS, S::SMEM, st>>>(p);
+    if (!first) return launch_after(skinny_kernel<MODE, COLS>, blocks, S::THREADS, S::SMEM, st, p);
+    skinny_kernel<MODE, COLS><<<blocks, S::THREADS, S::SMEM, st>>>(p);
     return cudaGetLastError();
+}
+template <int MODE>
+cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* hidden, int esz, long long width, long long stride, int num_sms,
+                          bool first, cudaStream_t st) {
+    if (cols == 16) return launch_skinny<MODE, 16>(p, hidden, esz, width, stride, num_sms, first, st);
+    if (cols == 32) return launch_skinny<MODE, 32>(p, hidden, esz, width, stride, num_sms, first, st);
+    if constexpr (MODE == FP8) {
+        if (cols == 128) return launch_skinny<MODE, 128>(p, hidden, esz, width, stride, num_sms, first, st);
+    }
+    return launch_skinny<MODE, 64>(p, hidden, esz, width, stride, num_sms, first, st);
 }
 
 constexpr int LSE_SLICE = 16;       // K blocks of 64: sums of 1024 products
-constexpr int HEAD_SKINNY_ROWS = 32;
+// Measured on both sides (V 151936; few-row kernel against the pair's, us):
+// loss, D 2048: 1 row 104 / 149, 32 rows 113 / 123, 64 rows 115 / 124, 128
+// rows 156 / 129. 8-bit product, K 4096: 1 row 110 / 197, 64 rows 148 / 189,
+// 128 rows 201 / 202 (V 32000, K 2048: 32 / 35), 256 rows 348 / 212.
+constexpr int HEAD_SKINNY_ROWS = 64;
 constexpr int FP8_SKINNY_ROWS = 128;
 
 // Partial sums a row's logits come in.
@@ -1507,8 +1525,7 @@ extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream
         p.part = part;
         p.target_logit = target_logit;
         parts = 4 * (a->num_sms < p.jobs ? a->num_sms : p.jobs);
-        e = cols == 16 ? launch_skinny<LSE, 16>(p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, true, st)
-                       : launch_skinny<LSE, 32>(p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, true, st);
+        e = launch_skinny<LSE>(cols, p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, true, st);
     } else {
         Params p = {};
         e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
@@ -1572,8 +1589,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             f.grad = a->grad_loss;
             f.dz = dz;
             f.dz_pitch = g.piece;
-            e = cols == 16 ? launch_skinny<DZ, 16>(f, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, q == 0, st)
-                           : launch_skinny<DZ, 32>(f, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, q == 0, st);
+            e = launch_skinny<DZ>(cols, f, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, q == 0, st);
         } else {
             e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
             if (e == cudaSuccess) e = make_map(&p.b, weight, 2, pw, a->D, a->weight_stride, 128);
@@ -1639,12 +1655,7 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
         p.out = a->out;
         p.out_stride = a->out_stride;
         p.out_bf16 = a->out_bf16;
-        switch (cols) {
-            case 16: return launch_skinny<FP8, 16>(p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
-            case 32: return launch_skinny<FP8, 32>(p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
-            case 64: return launch_skinny<FP8, 64>(p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
-            default: return launch_skinny<FP8, 128>(p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
-        }
+        return launch_skinny<FP8>(cols, p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
     }
     WideParams p = {};
     cudaError_t e = make_map(&p.a, a->x, 1, a->M, a->K, a->x_stride, 128);
