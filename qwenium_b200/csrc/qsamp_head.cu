@@ -826,15 +826,15 @@ __device__ __forceinline__ void take(uint32_t addr, float (&sum)[COLS], const fl
         tmem_wait_load(v);
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-            float4 x = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
             if (MODE == FP8) {
-                x = *(const float4*)(sx + c + i);
-                x.x *= sw, x.y *= sw, x.z *= sw, x.w *= sw;
+                const ulonglong2 x = *(const ulonglong2*)(sx + c + i);
+                fma2(Two(v[i], v[i + 1]), mul2(Two((uint64_t)x.x), Two(sw)), Two(sum[c + i], sum[c + i + 1])).get(sum[c + i], sum[c + i + 1]);
+                fma2(Two(v[i + 2], v[i + 3]), mul2(Two((uint64_t)x.y), Two(sw)), Two(sum[c + i + 2], sum[c + i + 3]))
+                    .get(sum[c + i + 2], sum[c + i + 3]);
+            } else {
+#pragma unroll
+                for (int q = i; q < i + 4; ++q) sum[c + q] += v[q];
             }
-            sum[c + i] = fmaf(v[i], x.x, sum[c + i]);
-            sum[c + i + 1] = fmaf(v[i + 1], x.y, sum[c + i + 1]);
-            sum[c + i + 2] = fmaf(v[i + 2], x.z, sum[c + i + 2]);
-            sum[c + i + 3] = fmaf(v[i + 3], x.w, sum[c + i + 3]);
         }
     }
 }
