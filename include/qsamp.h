@@ -326,7 +326,8 @@ qsamp_status qsamp_verify_greedy(qsamp_ctx* ctx, const void* logits, qsamp_dtype
  *   z[n][v]  = hidden[n] . weight[v],  l = z, or softcap * tanh(z / softcap)
  *   lse[n]   = log sum_v exp l[n][v],  loss[n] = lse[n] - l[n][targets[n]]
  * A row with a negative target has loss 0 and no gradient (its lse is still
- * written); a target >= V gives loss NaN and no gradient. -loss is the
+ * written), whatever its hidden row holds, NaN included; a target >= V gives
+ * loss NaN and no gradient. -loss is the
  * token's log-probability (logprobs of generated tokens, prompt scoring).
  * A logit of +infinity or NaN makes its row's results NaN.
  *

@@ -1092,6 +1092,21 @@ __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* part, cons
     }
 }
 
+// The hidden rows as d_weight's sums take them: zeros where a row has no
+// gradient, so that whatever lies there (padding, an infinity, a NaN) does not
+// meet its zero dz.
+__global__ void __launch_bounds__(256) live_rows_kernel(const uint16_t* hidden, long long stride, const int32_t* targets, int N,
+                                                        int D, int V, uint16_t* out) {
+    const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+    launch_next();
+    if (i >= (long long)N * D) return;
+    const long long row = i / D;
+    const int t = targets[row];
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (t >= 0 && t < V) w = *(const uint4*)(hidden + row * stride + i % D);
+    *(uint4*)(out + i) = w;
+}
+
 // d_hidden = the slabs' sum in their order, rounded once; eight columns a thread.
 __global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int splits, int N, int D, uint16_t* dh,
                                                       long long dh_stride) {
@@ -1457,12 +1472,13 @@ long long lse_parts(int N, int V, int num_sms) {
 // vocabulary. Few rows make few d_hidden tiles with a long sum; the splits are
 // the number for which the busiest pair has least to do. Job i runs on pair i
 // mod pairs, d_hidden's first: r pairs have one d_hidden job more, and the
-// d_weight jobs left over go to the pairs from r on.
+// d_weight jobs left over go to the pairs from r on. Every split's slab is read
+// and written per piece, so there are at most four jobs a pair of them.
 constexpr long long DZ_BYTES = 256ll << 20;
 constexpr int MAX_SPLITS = 32;
 struct GradPlan {
     int piece, pieces, splits;
-    long long dz_bytes, slab_bytes;
+    long long dz_bytes, slab_bytes, rows_bytes;
 };
 GradPlan grad_plan(int N, int V, int D, int num_sms) {
     GradPlan g;
@@ -1472,12 +1488,12 @@ GradPlan grad_plan(int N, int V, int D, int num_sms) {
     g.piece = (int)(ceil_div(ceil_div(V, g.pieces), TILE) * TILE);
     g.pieces = (int)ceil_div(V, g.piece);
     const long long dt = ceil_div(D, TILE), tiles = ceil_div(N, TILE) * dt, kb = ceil_div(g.piece, 64), pairs = num_sms / 2;
-    // in K blocks; a tile's epilogue that nothing hides costs about two
+    // in K blocks; a d_weight tile's epilogue that nothing hides costs about two, a slab's traffic about six
     const long long dw = ceil_div(g.piece, TILE) * dt, dw_cost = ceil_div(N, 64) + 2, dw_each = dw / pairs, dw_left = dw % pairs;
     long long best = INT64_MAX;
     g.splits = 1;
-    for (long long s = 1; s <= MAX_SPLITS && s * 8 <= kb; ++s) {
-        const long long cost = ceil_div(kb, s) + 2, each = tiles * s / pairs, r = tiles * s % pairs;
+    for (long long s = 1; s == 1 || (s <= MAX_SPLITS && s * 8 <= kb && s * tiles <= 4 * pairs); ++s) {
+        const long long cost = ceil_div(kb, s) + 6, each = tiles * s / pairs, r = tiles * s % pairs;
         long long worst = each * cost + (dw_each + (dw_left > 0)) * dw_cost;
         const long long more = r ? (each + 1) * cost + (dw_each + (dw_left > pairs - r)) * dw_cost : 0;
         if (more > worst) worst = more;
@@ -1488,6 +1504,7 @@ GradPlan grad_plan(int N, int V, int D, int num_sms) {
     }
     g.dz_bytes = al(2ll * N * g.piece);
     g.slab_bytes = al(4ll * g.splits * N * D);
+    g.rows_bytes = al(2ll * N * D);
     return g;
 }
 
@@ -1502,7 +1519,7 @@ extern "C" long long qs_head_loss_ws(int N, int V, int, int num_sms) {
 
 extern "C" long long qs_head_grad_ws(int N, int V, int D, int num_sms) {
     const GradPlan g = grad_plan(N, V, D, num_sms);
-    return g.dz_bytes + g.slab_bytes;
+    return g.dz_bytes + g.slab_bytes + g.rows_bytes;
 }
 
 extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream_t st) {
@@ -1559,11 +1576,15 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
     const GradPlan g = grad_plan(a->N, a->V, a->D, a->num_sms);
     uint16_t* dz = (uint16_t*)a->ws;
     float* slabs = (float*)(a->ws + g.dz_bytes);
+    uint16_t* rows = (uint16_t*)(a->ws + g.dz_bytes + g.slab_bytes);
+    const long long n = (long long)a->N * a->D / 8;
+    live_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(a->hidden, a->hidden_stride, a->targets, a->N, a->D, a->V, rows);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
     const int cols = skinny_cols(a->N, HEAD_SKINNY_ROWS);
     for (int q = 0; q < g.pieces; ++q) {
         const int p0 = q * g.piece, pw = a->V - p0 < g.piece ? a->V - p0 : g.piece;
         const uint16_t* weight = a->weight + (long long)p0 * a->weight_stride;
-        cudaError_t e;
         Params p = {};
         p.m_tiles = (int)ceil_div(a->N, TILE);
         p.n_tiles = (int)ceil_div(pw, TILE);
@@ -1589,7 +1610,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             f.grad = a->grad_loss;
             f.dz = dz;
             f.dz_pitch = g.piece;
-            e = launch_skinny<DZ>(cols, f, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, q == 0, st);
+            e = launch_skinny<DZ>(cols, f, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, false, st);
         } else {
             e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
             if (e == cudaSuccess) e = make_map(&p.b, weight, 2, pw, a->D, a->weight_stride, 128);
@@ -1603,13 +1624,13 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             p.softcap = a->softcap;
             p.lse = a->lse;
             p.grad = a->grad_loss;
-            e = launch<DZ>(p, a->num_sms, q == 0, st);
+            e = launch<DZ>(p, a->num_sms, false, st);
         }
         if (e != cudaSuccess) return e;
         e = make_map(&p.a, dz, 2, a->N, pw, g.piece, 128);
         if (e == cudaSuccess) e = make_map(&p.b, a->weight, 2, a->V, a->D, a->weight_stride, 64);
         if (e == cudaSuccess) e = make_map(&p.a2, dz, 2, a->N, pw, g.piece, 64);
-        if (e == cudaSuccess) e = make_map(&p.b2, a->hidden, 2, a->N, a->D, a->hidden_stride, 64);
+        if (e == cudaSuccess) e = make_map(&p.b2, rows, 2, a->N, a->D, a->D, 64);
         if (e == cudaSuccess)
             e = make_map(&p.o, a->d_weight + (long long)p0 * a->d_weight_stride, 2, pw, a->D, a->d_weight_stride, 32);
         if (e != cudaSuccess) return e;
@@ -1629,8 +1650,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         if (e != cudaSuccess) return e;
         *launches += 2;
     }
-    const long long n = (long long)a->N * a->D / 8;
-    *launches += 1;
+    *launches += 2;
     return launch_after(dh_join_kernel, ceil_div(n, 256), 256, 0, st, (const float*)slabs, g.splits, a->N, a->D, a->d_hidden,
                         a->d_hidden_stride);
 }

@@ -121,6 +121,26 @@ def test_rows_without_a_loss(torch, ctx):
     assert (dh == 0).all() and (dw == 0).all()
 
 
+@pytest.mark.parametrize("N", [20, 150])
+def test_whatever_lies_in_masked_rows(torch, ctx, N):
+    """NaN and infinities in hidden rows without a gradient (padding behind a
+    batch's sequences) reach no other row and not the weight's gradient."""
+    h, w, t, g = H.head_inputs(N, 700, 64, seed=15, ignored=0.4, device="cuda")
+    t[5] = 700  # past the vocabulary: no gradient either
+    dead = (t < 0) | (t >= 700)
+    want = H.head_exact(torch.where(dead[:, None], 0.0, h), w, t, g, 0.0)
+    bad = h.clone()
+    bad[dead] = torch.tensor([float("nan"), float("inf"), -float("inf"), 3e38], device="cuda").repeat(16).to(torch.bfloat16)
+    loss, lse = ctx.head_loss(bad, w, t)
+    keep = t >= 700
+    assert (loss[dead & ~keep] == 0).all()
+    within(loss[~dead], want["loss"][~dead], want["eloss"][~dead], "loss")
+    dh, dw = ctx.head_loss_grad(bad, w, t, lse, torch.where(dead, float("nan"), g))
+    assert (dh[dead] == 0).all()
+    within(dh, want["dh"], want["edh"], "d_hidden")
+    within(dw, want["dw"], want["edw"], "d_weight")
+
+
 def test_no_rows(torch, ctx):
     _, w, _, _ = H.head_inputs(1, 300, 64, device="cuda")
     h = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda")
