@@ -1334,6 +1334,14 @@ static qsamp_status check_matrix(qsamp_ctx* c, const char* name, const void* p, 
     return QSAMP_OK;
 }
 
+// Coordinates of a tile's end stay in 32 bits.
+constexpr int32_t kMaxExtent = 1 << 30;
+static qsamp_status check_extent(qsamp_ctx* c, const char* name, int32_t n, int32_t least) {
+    if (n < least) return fail(c, QSAMP_ERR_INVALID_ARG, "%s: expected >= %d, got %d", name, least, n);
+    if (n > kMaxExtent) return fail(c, QSAMP_ERR_UNSUPPORTED, "%s: expected <= %d, got %d", name, kMaxExtent, n);
+    return QSAMP_OK;
+}
+
 // Tiles are numbered in 32 bits.
 static qsamp_status check_tiles(qsamp_ctx* c, int64_t rows, int64_t cols) {
     if (((rows + 63) / 64) * ((cols + 63) / 64) > INT32_MAX)
@@ -1345,16 +1353,17 @@ static qsamp_status check_tiles(qsamp_ctx* c, int64_t rows, int64_t cols) {
 static qsamp_status head_call(qsamp_ctx* c, const qsamp_head* h, int grad, void* workspace, int64_t workspace_bytes,
                               qs::HeadCall& a) {
     if (!h) return fail(c, QSAMP_ERR_INVALID_ARG, "head: expected non-NULL");
-    if (h->N < 0) return fail(c, QSAMP_ERR_INVALID_ARG, "N: expected >= 0, got %d", h->N);
-    if (h->V < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "V: expected >= 1, got %d", h->V);
-    if (h->D < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "D: expected >= 1, got %d", h->D);
+    qsamp_status s = check_extent(c, "N", h->N, 0);
+    if (s == QSAMP_OK) s = check_extent(c, "V", h->V, 1);
+    if (s == QSAMP_OK) s = check_extent(c, "D", h->D, 1);
+    if (s != QSAMP_OK) return s;
     if (h->D % 8 != 0) return fail(c, QSAMP_ERR_UNSUPPORTED, "D: expected a multiple of 8, got %d", h->D);
     if (!(h->softcap >= 0.0f) || std::isinf(h->softcap))
         return fail(c, QSAMP_ERR_INVALID_ARG, "softcap: expected a number >= 0, got %g", h->softcap);
     if (!h->weight) return fail(c, QSAMP_ERR_INVALID_ARG, "weight: expected non-NULL");
     if (h->N > 0 && (!h->hidden || !h->targets))
         return fail(c, QSAMP_ERR_INVALID_ARG, "hidden / targets: expected non-NULL");
-    qsamp_status s = check_matrix(c, "hidden", h->hidden, h->hidden_stride, h->D, 2);
+    s = check_matrix(c, "hidden", h->hidden, h->hidden_stride, h->D, 2);
     if (s == QSAMP_OK) s = check_matrix(c, "weight", h->weight, h->weight_stride, h->D, 2);
     if (s == QSAMP_OK) s = check_tiles(c, h->N, h->V);
     if (s == QSAMP_OK) s = check_tiles(c, h->N, h->D);
@@ -1444,16 +1453,15 @@ qsamp_status qsamp_quantize_fp8(qsamp_ctx* c, const void* x, qsamp_dtype dtype, 
     std::lock_guard<std::mutex> g(c->mu);
     if (dtype != QSAMP_F32 && dtype != QSAMP_BF16)
         return fail(c, QSAMP_ERR_INVALID_ARG, "dtype: expected QSAMP_F32 or QSAMP_BF16, got %d", (int)dtype);
-    if (M < 0) return fail(c, QSAMP_ERR_INVALID_ARG, "M: expected >= 0, got %d", M);
-    if (K < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "K: expected >= 1, got %d", K);
+    qsamp_status s = check_extent(c, "M", M, 0);
+    if (s == QSAMP_OK) s = check_extent(c, "K", K, 1);
+    if (s != QSAMP_OK) return s;
     if (block_rows != 1 && block_rows != qs::FP8_BLOCK)
         return fail(c, QSAMP_ERR_INVALID_ARG, "block_rows: expected 1 or %d, got %d", qs::FP8_BLOCK, block_rows);
     const int64_t kb = qs::ceil_div(K, qs::FP8_BLOCK);
     if (x_stride < K || q_stride < K || scale_stride < kb)
         return fail(c, QSAMP_ERR_INVALID_ARG, "x / q / scale stride: expected >= %d / %d / %lld, got %lld / %lld / %lld", K,
                     K, (long long)kb, (long long)x_stride, (long long)q_stride, (long long)scale_stride);
-    if ((int64_t)M * kb > (int64_t)INT32_MAX * 8)
-        return fail(c, QSAMP_ERR_UNSUPPORTED, "%d x %d: more blocks than one launch numbers", M, K);
     if (M == 0) return QSAMP_OK;
     if (!x || !q || !scale) return fail(c, QSAMP_ERR_INVALID_ARG, "x / q / scale: expected non-NULL");
     return on_device(c, "quantisation launch", [&](int* n) {
@@ -1467,9 +1475,10 @@ qsamp_status qsamp_matmul_fp8(qsamp_ctx* c, const qsamp_fp8_product* p, void* st
     if (!c) return QSAMP_ERR_INVALID_ARG;
     std::lock_guard<std::mutex> g(c->mu);
     if (!p) return fail(c, QSAMP_ERR_INVALID_ARG, "product: expected non-NULL");
-    if (p->M < 0) return fail(c, QSAMP_ERR_INVALID_ARG, "M: expected >= 0, got %d", p->M);
-    if (p->V < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "V: expected >= 1, got %d", p->V);
-    if (p->K < 1) return fail(c, QSAMP_ERR_INVALID_ARG, "K: expected >= 1, got %d", p->K);
+    qsamp_status s = check_extent(c, "M", p->M, 0);
+    if (s == QSAMP_OK) s = check_extent(c, "V", p->V, 1);
+    if (s == QSAMP_OK) s = check_extent(c, "K", p->K, 1);
+    if (s != QSAMP_OK) return s;
     if (p->out_dtype != QSAMP_F32 && p->out_dtype != QSAMP_BF16)
         return fail(c, QSAMP_ERR_INVALID_ARG, "out_dtype: expected QSAMP_F32 or QSAMP_BF16, got %d", (int)p->out_dtype);
     const int64_t kb = qs::ceil_div(p->K, qs::FP8_BLOCK);
@@ -1481,7 +1490,7 @@ qsamp_status qsamp_matmul_fp8(qsamp_ctx* c, const qsamp_fp8_product* p, void* st
     if (p->M == 0) return QSAMP_OK;
     if (!p->x || !p->w || !p->x_scale || !p->w_scale || !p->out)
         return fail(c, QSAMP_ERR_INVALID_ARG, "x / w / x_scale / w_scale / out: expected non-NULL");
-    qsamp_status s = check_matrix(c, "x", p->x, p->x_stride, p->K, 1);
+    s = check_matrix(c, "x", p->x, p->x_stride, p->K, 1);
     if (s == QSAMP_OK) s = check_matrix(c, "w", p->w, p->w_stride, p->K, 1);
     if (s == QSAMP_OK) s = check_tiles(c, p->M, p->V);
     if (s != QSAMP_OK) return s;

@@ -1129,7 +1129,7 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
     return r;
 }
 
-// What quantising by a scale needs: -s, 1 / s (to half a step), (2^19 + 1) / s
+// What quantising by a scale needs: -s, 1 / s (to a step), (2^19 + 1) / s
 // and 2^38 / s.
 struct Quotient {
     Two minus_s, inv, inv_split;
@@ -1160,16 +1160,23 @@ __device__ __forceinline__ void round_as_quotients(float& a, float& b, const Quo
     fma2(side, Two(3.0f * 0x1p-16f), h).get(a, b);
 }
 
-// A quantisation block's scale and its reciprocal; top: the block's largest
-// magnitude as bits (an infinity or a NaN: NaN for all).
-struct BlockScale {
-    float s, inv;
-};
-__device__ __forceinline__ BlockScale block_scale(uint32_t top) {
-    BlockScale b;
-    b.s = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 448.0f) : NAN;
-    b.inv = __frcp_rn(b.s);
-    return b;
+// A quantisation block's scale, the largest magnitude (top, as bits; an
+// infinity or a NaN: NaN for all) over 448 rounded once. In the range of
+// quantize8: the product with 1/448, corrected by its exact remainder
+// (P. Markstein, IBM J. Res. Develop. 34(1), 1990; every mantissa is tested),
+// in a quarter of a division's instructions.
+constexpr float SMALL_SCALE = 0x1p-60f;
+__device__ __forceinline__ float block_scale(uint32_t top) {
+    const float t = __uint_as_float(top), r = 1.0f / 448.0f, q = t * r;
+    const float s = fmaf(fmaf(-q, 448.0f, t), r, q);
+    if (s >= SMALL_SCALE && top < 0x7f800000u) return s;
+    return top < 0x7f800000u ? __fdiv_rn(t, 448.0f) : NAN;
+}
+// 1 / s to a step, for s in that range.
+__device__ __forceinline__ float reciprocal(float s) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    return r;
 }
 
 __device__ __forceinline__ uint2 quantize8(float (&x)[8], const Quotient& q) {
@@ -1181,14 +1188,13 @@ __device__ __forceinline__ uint2 quantize8(float (&x)[8], const Quotient& q) {
     return make_uint2(w[0], w[1]);
 }
 
-// Scales whose reciprocals or remainders leave the range, and none: NaN.
-constexpr float SMALL_SCALE = 0x1p-60f;
+// Scales whose reciprocals or remainders leave the range, and NaN.
 __device__ __forceinline__ uint2 quantize8_small(float (&x)[8], float s) {
     if (s > 0.0f) {  // lifted by an exact power of two
         s *= 0x1p100f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] *= 0x1p100f;
-        return quantize8(x, Quotient(s, __frcp_rn(s)));
+        return quantize8(x, Quotient(s, reciprocal(s)));
     }
     uint32_t w[2] = {0, 0};
 #pragma unroll
@@ -1252,12 +1258,14 @@ __device__ __forceinline__ void store8(uint8_t* row, int k, int K, bool vec, uin
     }
 }
 
-// Blocks of one row: 16 threads a block, eight values a thread; a warp takes
-// 256 columns of four rows with all their loads in flight, and eight of its
-// lanes make the eight blocks' scales. Each value is read once and held in
-// registers between the maximum and the quotients. FULL: whole blocks and
-// whole groups of rows on aligned addresses, without checks per value.
-constexpr int QROWS = 4;
+// Blocks of one row: eight threads a block, sixteen values a thread (two
+// pieces, so that a load's lanes are neighbours); a warp takes 512 columns of
+// four rows with all their loads in flight. Each value is read once and held
+// in registers between the maximum and the quotients. FULL: whole blocks and
+// whole groups of rows on aligned addresses, without checks per value (which
+// would cost registers, and a quarter of the rate). A CTA's warps lie below
+// each other, so that the few slower ones at the right edge share CTAs.
+constexpr int QROWS = 4, QCOLS = 512;
 struct QuantArgs {
     const void* x;
     uint8_t* q;
@@ -1266,48 +1274,49 @@ struct QuantArgs {
     int M, K, x_vec, q_vec;
 };
 template <typename T, bool FULL>
-__device__ __forceinline__ void quantize_rows(const QuantArgs& a, int m0, int k) {
-    const int lane = threadIdx.x % 32;
+__device__ __forceinline__ void quantize_rows(const QuantArgs& a, int m0, int k0) {
+    const int lane = threadIdx.x % 32, k = k0 + lane / 8 * FP8_BLOCK + lane % 8 * 8;
+    const int last = FULL ? INT32_MAX : a.K;
     const T* x = (const T*)a.x + m0 * a.x_stride;
-    Eight<T> e[QROWS];
-#pragma unroll
-    for (int r = 0; r < QROWS; ++r)
-        e[r].load(x + (FULL ? r : min(r, a.M - 1 - m0)) * a.x_stride, k, FULL ? INT32_MAX : a.K, FULL || a.x_vec);
-    uint32_t mine = 0;
+    Eight<T> e[QROWS][2];
 #pragma unroll
     for (int r = 0; r < QROWS; ++r) {
-        uint32_t top = e[r].top();
-#pragma unroll
-        for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (lane % QROWS == r) mine = top;
+        e[r][0].load(x, k, last, FULL || a.x_vec);
+        e[r][1].load(x, k + 64, last, FULL || a.x_vec);
+        if (FULL || m0 + r + 1 < a.M) x += a.x_stride;
     }
-    const BlockScale b = block_scale(mine);
-    // lane r of a block's sixteen holds row r's scale
-    const int row = lane % 16, kb = k / FP8_BLOCK;
-    if (row < QROWS && m0 + row < a.M && kb * FP8_BLOCK < a.K) a.scale[(m0 + row) * a.scale_stride + kb] = b.s;
     uint8_t* q = a.q + m0 * a.q_stride;
+    float* scale = a.scale + m0 * a.scale_stride + k / FP8_BLOCK;
 #pragma unroll
     for (int r = 0; r < QROWS; ++r) {
-        const float s = __shfl_sync(0xffffffffu, b.s, (lane & 16) + r), inv = __shfl_sync(0xffffffffu, b.inv, (lane & 16) + r);
-        if (FULL || (m0 + r < a.M && k < a.K)) {
-            float v[8];
-            e[r].values(v);
-            store8(q + r * a.q_stride, k, FULL ? INT32_MAX : a.K, FULL || a.q_vec,
-                   s >= SMALL_SCALE ? quantize8(v, Quotient(s, inv)) : quantize8_small(v, s));
+        uint32_t top = max(e[r][0].top(), e[r][1].top());
+#pragma unroll
+        for (int o = 4; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float s = block_scale(top);
+        if (FULL || m0 + r < a.M) {
+            if (lane % 8 == 0 && (FULL || k < a.K)) *scale = s;
+            const Quotient quotient(s, reciprocal(s));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+                e[r][h].values(v);
+                if (FULL || k + 64 * h < a.K)
+                    store8(q, k + 64 * h, last, FULL || a.q_vec, s >= SMALL_SCALE ? quantize8(v, quotient) : quantize8_small(v, s));
+            }
         }
+        q += a.q_stride;
+        scale += a.scale_stride;
     }
 }
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a, int groups, int log_across) {
-    // a block's eight warps: 2^log_across of them along a row
-    const int warp = threadIdx.x / 32, down = 8 >> log_across;
-    const long long m0 = ((long long)(blockIdx.x / groups) * down + (warp >> log_across)) * QROWS;
-    const int k0 = ((blockIdx.x % groups << log_across) + (warp & ((1 << log_across) - 1))) * 256;
-    if (m0 >= a.M) return;
-    if (a.x_vec && a.q_vec && m0 + QROWS <= a.M && k0 + 256 <= a.K)
-        quantize_rows<T, true>(a, (int)m0, k0 + threadIdx.x % 32 * 8);
-    else
-        quantize_rows<T, false>(a, (int)m0, k0 + threadIdx.x % 32 * 8);
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
+    const int k0 = blockIdx.x * QCOLS;
+    for (long long m0 = ((long long)blockIdx.y * 8 + threadIdx.x / 32) * QROWS; m0 < a.M; m0 += (long long)gridDim.y * 8 * QROWS) {
+        if (a.x_vec && a.q_vec && m0 + QROWS <= a.M && k0 <= a.K - QCOLS)
+            quantize_rows<T, true>(a, (int)m0, k0);
+        else
+            quantize_rows<T, false>(a, (int)m0, k0);
+    }
 }
 
 // Blocks of 128 x 128: one CTA each, eight rows' values a thread held in
@@ -1316,11 +1325,15 @@ template <typename T, bool FULL>
 __device__ __forceinline__ void quantize_square(const QuantArgs& a, int mb, int kb) {
     __shared__ uint32_t red[8];
     const int m0 = mb * FP8_BLOCK + threadIdx.x / 16, k = kb * FP8_BLOCK + threadIdx.x % 16 * 8;
-    const T* x = (const T*)a.x;
+    const int last = FULL ? INT32_MAX : a.K;
+    const T* x = (const T*)a.x + (FULL ? m0 : min(m0, a.M - 1)) * a.x_stride;
+    const long long x_step = 16 * a.x_stride, q_step = 16 * a.q_stride;
     Eight<T> e[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-        e[r].load(x + (FULL ? m0 + 16 * r : min(m0 + 16 * r, a.M - 1)) * a.x_stride, k, FULL ? INT32_MAX : a.K, FULL || a.x_vec);
+    for (int r = 0; r < 8; ++r) {
+        e[r].load(x, k, last, FULL || a.x_vec);
+        if (FULL || m0 + 16 * (r + 1) < a.M) x += x_step;
+    }
     uint32_t top = 0;
 #pragma unroll
     for (int r = 0; r < 8; ++r) top = max(top, e[r].top());
@@ -1329,29 +1342,31 @@ __device__ __forceinline__ void quantize_square(const QuantArgs& a, int mb, int 
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, red[i]);
-    const BlockScale b = block_scale(top);
-    if (threadIdx.x == 0) a.scale[mb * a.scale_stride + kb] = b.s;
-    if (!FULL && k >= a.K) return;
-    const Quotient quotient(b.s, b.inv);
+    const float s = block_scale(top);
+    if (threadIdx.x == 0) a.scale[mb * a.scale_stride + kb] = s;
+    const Quotient quotient(s, reciprocal(s));
     uint8_t* q = a.q + m0 * a.q_stride;
-    const bool small = !(b.s >= SMALL_SCALE);
+    const bool small = !(s >= SMALL_SCALE);
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-        if (FULL || m0 + 16 * r < a.M) {
+        if (FULL || (m0 + 16 * r < a.M && k < a.K)) {
             float v[8];
             e[r].values(v);
-            store8(q + 16 * r * a.q_stride, k, FULL ? INT32_MAX : a.K, FULL || a.q_vec,
-                   small ? quantize8_small(v, b.s) : quantize8(v, quotient));
+            store8(q, k, last, FULL || a.q_vec, small ? quantize8_small(v, s) : quantize8(v, quotient));
         }
+        q += q_step;
     }
+    __syncthreads();  // red is free for the next block
 }
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_square_kernel(const QuantArgs a) {
-    const int per_row = (a.K + FP8_BLOCK - 1) / FP8_BLOCK, kb = blockIdx.x % per_row, mb = blockIdx.x / per_row;
-    if (a.x_vec && a.q_vec && (long long)(mb + 1) * FP8_BLOCK <= a.M && (long long)(kb + 1) * FP8_BLOCK <= a.K)
-        quantize_square<T, true>(a, mb, kb);
-    else
-        quantize_square<T, false>(a, mb, kb);
+    const int kb = blockIdx.x, blocks = (a.M - 1) / FP8_BLOCK + 1;
+    for (int mb = blockIdx.y; mb < blocks; mb += gridDim.y) {
+        if (a.x_vec && a.q_vec && mb < a.M / FP8_BLOCK && kb < a.K / FP8_BLOCK)
+            quantize_square<T, true>(a, mb, kb);
+        else
+            quantize_square<T, false>(a, mb, kb);
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -1705,14 +1720,11 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
 
 template <typename T>
 static cudaError_t quantize(const QuantArgs& a, int block_rows, cudaStream_t st) {
-    if (block_rows == 1) {
-        int log_across = 0;
-        while (log_across < 3 && (256 << log_across) < a.K) ++log_across;
-        const long long groups = ceil_div(a.K, 256 << log_across), down = ceil_div(a.M, QROWS * (8 >> log_across));
-        quantize_rows_kernel<T><<<(unsigned)(groups * down), 256, 0, st>>>(a, (int)groups, log_across);
-    } else {
-        quantize_square_kernel<T><<<(unsigned)(ceil_div(a.M, FP8_BLOCK) * ceil_div(a.K, FP8_BLOCK)), 256, 0, st>>>(a);
-    }
+    const auto grid = [](long long x, long long y) { return dim3((unsigned)x, (unsigned)(y < 65535 ? y : 65535)); };
+    if (block_rows == 1)
+        quantize_rows_kernel<T><<<grid(ceil_div(a.K, QCOLS), ceil_div(a.M, QROWS * 8)), 256, 0, st>>>(a);
+    else
+        quantize_square_kernel<T><<<grid(ceil_div(a.K, FP8_BLOCK), ceil_div(a.M, FP8_BLOCK)), 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 

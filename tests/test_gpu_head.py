@@ -293,6 +293,17 @@ def test_quantiser_every_bf16(torch, ctx):
         assert torch.equal(q.double(), want), f"largest {top}: {int((q.double() != want).sum())} codes differ"
 
 
+@pytest.mark.parametrize("exponent", [0, 40, -45, 127])
+def test_scale_of_every_mantissa(torch, ctx, exponent):
+    """The scale is the largest value over 448, rounded once."""
+    bits = torch.arange(2**23, dtype=torch.int32, device="cuda") | ((exponent + 127) << 23)
+    x = bits.view(torch.float32).reshape(-1, 1)
+    q, s = ctx.quantize_fp8(x)
+    want = x.double() / torch.full_like(x, 448.0, dtype=torch.float64)  # 53 bits: 24 of them over 7 need no second look
+    assert torch.equal(s, want.float())
+    assert (q.float() == 448).all()
+
+
 @pytest.mark.parametrize("rows", [1, 128])
 def test_quantiser_large(torch, ctx, rows):
     """Random values over many binades in blocks of both shapes, both types."""
