@@ -805,7 +805,7 @@ struct SkinnyParams {
     float* target_logit;
     const float* lse;     // DZ
     const float* grad;
-    uint16_t* dz;         // DZ: [M][dz_pitch]: the V vocabulary columns from n0
+    uint16_t* dz;         // DZ: [2 M][dz_pitch]: the V vocabulary columns from n0, and below what rounding left
     long long dz_pitch;
     int n0, V_total;
     const float* sx;
@@ -996,7 +996,10 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
                     if (i < mine) {
                         const int at = ((const int*)table)[2 * COLS + c0 + i];
                         const float d = dz_of(sum[i], table[c0 + i], table[COLS + c0 + i], inv, at == v, at == INT32_MIN);
-                        ((__nv_bfloat16*)p.dz)[(c0 + i) * p.dz_pitch + v] = __float2bfloat16_rn(d);
+                        const __nv_bfloat16 high = __float2bfloat16_rn(d);
+                        __nv_bfloat16* out = (__nv_bfloat16*)p.dz + (c0 + i) * p.dz_pitch + v;
+                        out[0] = high;
+                        out[p.M * p.dz_pitch] = __float2bfloat16_rn(d - __bfloat162float(high));
                     }
                 }
             } else {
@@ -1094,27 +1097,28 @@ __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* part, cons
 
 // The hidden rows as d_weight's sums take them: zeros where a row has no
 // gradient, so that whatever lies there (padding, an infinity, a NaN) does not
-// meet its zero dz.
+// meet its zero dz; parts times one below the other.
 __global__ void __launch_bounds__(256) live_rows_kernel(const uint16_t* hidden, long long stride, const int32_t* targets, int N,
-                                                        int D, int V, uint16_t* out) {
-    const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+                                                        int D, int V, int parts, uint16_t* out) {
+    const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8, n = (long long)N * D;
     launch_next();
-    if (i >= (long long)N * D) return;
+    if (i >= n) return;
     const long long row = i / D;
     const int t = targets[row];
     uint4 w = make_uint4(0, 0, 0, 0);
     if (t >= 0 && t < V) w = *(const uint4*)(hidden + row * stride + i % D);
-    *(uint4*)(out + i) = w;
+    for (int q = 0; q < parts; ++q) *(uint4*)(out + q * n + i) = w;
 }
 
-// d_hidden = the slabs' sum in their order, rounded once; eight columns a thread.
-__global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int splits, int N, int D, uint16_t* dh,
+// d_hidden = the slabs' sum (and the parts' of each) in their order, rounded
+// once; eight columns a thread.
+__global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int slices, int N, int D, uint16_t* dh,
                                                       long long dh_stride) {
     const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8, n = (long long)N * D;
     if (i >= n) return;
     wait_previous();
     float v[8] = {};
-    for (int s = 0; s < splits; ++s) {
+    for (int s = 0; s < slices; ++s) {
         const float4 x = *(const float4*)(slabs + s * n + i), y = *(const float4*)(slabs + s * n + i + 4);
         v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
     }
@@ -1495,7 +1499,14 @@ struct GradPlan {
     int piece, pieces, splits;
     long long dz_bytes, slab_bytes, rows_bytes;
 };
-GradPlan grad_plan(int N, int V, int D, int num_sms) {
+// Few rows (the few-row kernel's) have their dz in two parts, the bf16 value
+// and what its rounding left: a row's largest term, its target's, would
+// otherwise put its one rounding error on the whole row of d_hidden and of
+// d_weight. Their products are bound by the weight's bytes and do not feel
+// the second part; with more rows the errors average out.
+int grad_parts(int N) { return skinny_cols(N, HEAD_SKINNY_ROWS) ? 2 : 1; }
+GradPlan grad_plan(int rows, int V, int D, int num_sms) {
+    const int N = rows * grad_parts(rows);
     GradPlan g;
     const long long most = (DZ_BYTES / 2 / (N > 0 ? N : 1)) / TILE * TILE;
     const long long cap = most < TILE ? TILE : most;
@@ -1592,8 +1603,10 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
     uint16_t* dz = (uint16_t*)a->ws;
     float* slabs = (float*)(a->ws + g.dz_bytes);
     uint16_t* rows = (uint16_t*)(a->ws + g.dz_bytes + g.slab_bytes);
+    const int parts = grad_parts(a->N), R = a->N * parts;
     const long long n = (long long)a->N * a->D / 8;
-    live_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(a->hidden, a->hidden_stride, a->targets, a->N, a->D, a->V, rows);
+    live_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(a->hidden, a->hidden_stride, a->targets, a->N, a->D, a->V, parts,
+                                                                 rows);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const int cols = skinny_cols(a->N, HEAD_SKINNY_ROWS);
@@ -1642,10 +1655,11 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             e = launch<DZ>(p, a->num_sms, false, st);
         }
         if (e != cudaSuccess) return e;
-        e = make_map(&p.a, dz, 2, a->N, pw, g.piece, 128);
+        p.m_tiles = (int)ceil_div(R, TILE);
+        e = make_map(&p.a, dz, 2, R, pw, g.piece, 128);
         if (e == cudaSuccess) e = make_map(&p.b, a->weight, 2, a->V, a->D, a->weight_stride, 64);
-        if (e == cudaSuccess) e = make_map(&p.a2, dz, 2, a->N, pw, g.piece, 64);
-        if (e == cudaSuccess) e = make_map(&p.b2, rows, 2, a->N, a->D, a->D, 64);
+        if (e == cudaSuccess) e = make_map(&p.a2, dz, 2, R, pw, g.piece, 64);
+        if (e == cudaSuccess) e = make_map(&p.b2, rows, 2, R, a->D, a->D, 64);
         if (e == cudaSuccess)
             e = make_map(&p.o, a->d_weight + (long long)p0 * a->d_weight_stride, 2, pw, a->D, a->d_weight_stride, 32);
         if (e != cudaSuccess) return e;
@@ -1654,10 +1668,10 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.dh_k_blocks = (int)ceil_div(pw, 64);
         // every split has a K block; a short last piece adds to the first slabs
         p.splits = g.splits < p.dh_k_blocks ? g.splits : p.dh_k_blocks;
-        p.dw_k_blocks = (int)ceil_div(a->N, 64);
+        p.dw_k_blocks = (int)ceil_div(R, 64);
         p.dh_jobs = p.m_tiles * p.d_tiles * p.splits;
         p.jobs = p.dh_jobs + p.n_tiles * p.d_tiles;
-        p.rows = a->N;
+        p.rows = R;
         p.D = a->D;
         p.slabs = slabs;
         p.add = q > 0;
@@ -1666,7 +1680,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         *launches += 2;
     }
     *launches += 2;
-    return launch_after(dh_join_kernel, ceil_div(n, 256), 256, 0, st, (const float*)slabs, g.splits, a->N, a->D, a->d_hidden,
+    return launch_after(dh_join_kernel, ceil_div(n, 256), 256, 0, st, (const float*)slabs, g.splits * parts, a->N, a->D, a->d_hidden,
                         a->d_hidden_stride);
 }
 

@@ -29,7 +29,7 @@ def head_inputs(N, V, D, seed=0, scale=3.0, ignored=0.2, device="cpu"):
     return tuple(x.to(device) for x in (h, w, t, grad))
 
 
-def head_exact(h, w, t, grad, cap):
+def head_exact(h, w, t, grad, cap, dz_error=U16):
     """64-bit loss, lse, dh, dw and the bounds of the bf16 / fp32 results.
 
     Logits: a sum of D products in 32 bits, in any order, is off by at most
@@ -38,7 +38,8 @@ def head_exact(h, w, t, grad, cap):
     exponentials (an argument rounded to U32 of at most 2^7, a 4 U32
     evaluation), sums of V terms in any order, one logarithm and the final
     rounding. dz is rounded to bf16; sums of the products in 32 bits;
-    the results rounded to bf16.
+    the results rounded to bf16. dz_error: dz's own rounding, U16 (few rows
+    have it in two parts: U16 squared).
     """
     N, D = h.shape
     V = w.shape[0]
@@ -63,7 +64,7 @@ def head_exact(h, w, t, grad, cap):
     gr = torch.where(live, grad.double(), 0.0).unsqueeze(1)
     dz = (p - hot) * slope * gr
     # a logit off by e moves p by p e, and the cap's slope by 2 e / cap
-    edz = U16 * dz.abs() + gr.abs() * slope.abs() * p * (ez + elsum.unsqueeze(1) + 2**-16)
+    edz = dz_error * dz.abs() + gr.abs() * slope.abs() * p * (ez + elsum.unsqueeze(1) + 2**-16)
     edz = edz + gr.abs() * (p + hot) * 8 * U32
     if cap > 0:
         edz = edz + gr.abs() * (p + hot) * (2 * ez / cap + 8 * U32)

@@ -51,7 +51,7 @@ SIZES = [
 @pytest.mark.parametrize("N,V,D", SIZES)
 def test_loss_and_gradients(torch, ctx, N, V, D, cap):
     h, w, t, g = H.head_inputs(N, V, D, seed=1, device="cuda")
-    want = H.head_exact(h, w, t, g, cap)
+    want = H.head_exact(h, w, t, g, cap, dz_error=H.U16**2 if N <= 64 else H.U16)
     loss, lse = ctx.head_loss(h, w, t, softcap=cap)
     within(loss, want["loss"], want["eloss"], "loss")
     within(lse, want["lse"], want["else"], "lse")
