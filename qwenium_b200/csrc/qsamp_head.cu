@@ -1473,7 +1473,13 @@ cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* hidden, int esz
     return launch_skinny<MODE, 64>(p, hidden, esz, width, stride, num_sms, first, st);
 }
 
-constexpr int LSE_SLICE = 16;       // K blocks of 64: sums of 1024 products
+// K blocks of 64 whose products are summed in tensor memory before fp32
+// registers take the sum. Tensor memory cuts each addition's last bits: the
+// lse comes out low by 0.5e-6 for every K block in a slice (0.9e-6, 3.8e-6,
+// 8e-6 measured at 2, 8, 16, whatever D). Shorter slices are free where the
+// weight's bytes bound the kernel; the pair's takes 2% more at 8 than at 16,
+// 13% at 4.
+constexpr int LSE_SLICE = 8, LSE_SKINNY_SLICE = 2;
 // Measured on both sides (V 151936; few-row kernel against the pair's, us):
 // loss, D 2048: 1 row 104 / 149, 32 rows 113 / 123, 64 rows 115 / 124, 128
 // rows 156 / 129. 8-bit product, K 4096: 1 row 110 / 197, 64 rows 148 / 189,
@@ -1560,7 +1566,7 @@ extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream
         p.V = a->V;
         p.M = a->N;
         p.k_blocks = (int)ceil_div(a->D, 64);
-        p.slice = LSE_SLICE;
+        p.slice = LSE_SKINNY_SLICE;
         p.jobs = (int)ceil_div(a->V, 128);
         p.status = a->status;
         p.targets = a->targets;
