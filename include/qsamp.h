@@ -122,7 +122,8 @@ qsamp_status qsamp_sample_host(qsamp_ctx* ctx, const qsamp_batch* batch);
  * carry token -1. The reference throws where a row cannot be sampled
  * (sampling.cpp:101,140): a caller that replaces Sampler::sample with
  * qsamp_sample converts QSAMP_ERR_DEVICE into that throw.
- * (qsamp_sample_host reads the status itself and returns it.) */
+ * (qsamp_sample_host reads the status itself and returns it.) A bounded wait
+ * that ran out in an output-head kernel is reported first, and once. */
 qsamp_status qsamp_poll_status(qsamp_ctx* ctx);
 
 /* Device-side limits of a context (no counterpart in the reference). The
