@@ -352,7 +352,7 @@ typedef struct qsamp_head {
     const int32_t* targets;  /* DEVICE [N]                       */
     int32_t N, V, D;
     int64_t hidden_stride, weight_stride; /* elements, >= D      */
-    float softcap;           /* 0: off                           */
+    float softcap;           /* 0: off; 2^-60 to 2^60            */
 } qsamp_head;
 int64_t qsamp_head_workspace(const qsamp_ctx* ctx, int32_t N, int32_t V, int32_t D, int32_t grad);
 qsamp_status qsamp_head_loss(qsamp_ctx* ctx, const qsamp_head* head, float* out_loss, float* out_lse, void* workspace,

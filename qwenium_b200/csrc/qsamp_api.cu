@@ -1358,8 +1358,8 @@ static qsamp_status head_call(qsamp_ctx* c, const qsamp_head* h, int grad, void*
     if (s == QSAMP_OK) s = check_extent(c, "D", h->D, 1);
     if (s != QSAMP_OK) return s;
     if (h->D % 8 != 0) return fail(c, QSAMP_ERR_UNSUPPORTED, "D: expected a multiple of 8, got %d", h->D);
-    if (!(h->softcap >= 0.0f) || std::isinf(h->softcap))
-        return fail(c, QSAMP_ERR_INVALID_ARG, "softcap: expected a number >= 0, got %g", h->softcap);
+    if (h->softcap != 0.0f && !(h->softcap >= 0x1p-60f && h->softcap <= 0x1p60f))
+        return fail(c, QSAMP_ERR_INVALID_ARG, "softcap: expected 0 or a number from 2^-60 to 2^60, got %g", h->softcap);
     if (!h->weight) return fail(c, QSAMP_ERR_INVALID_ARG, "weight: expected non-NULL");
     if (h->N > 0 && (!h->hidden || !h->targets))
         return fail(c, QSAMP_ERR_INVALID_ARG, "hidden / targets: expected non-NULL");

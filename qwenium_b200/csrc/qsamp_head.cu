@@ -135,15 +135,27 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
 }
 
 // ---------------------------------------------------------------- epilogues
-// One thread's view of a tile: its row, and how to store 32 columns of it.
+// cap tanh(z / cap) = cap (1 - 2 / (exp(2 z / cap) + 1)): the absolute error is
+// a few 2^-24 of cap, and the exponential's overflow gives the limit. A cap
+// above 64 would lose small logits in that, so there tanh's series to y^9
+// serves |z / cap| < 1/4 (it takes 6% of the loss's time, 256 x 2048 x 262144;
+// at a cap of 30 the plain form is within 1e-5).
 template <int N>
 __device__ __forceinline__ void logits_of(float (&v)[N], float cap) {
-    // cap tanh(z / cap) = cap (1 - 2 / (exp(2 z / cap) + 1)): absolute error a
-    // few 2^-24 of cap, and the exponential's overflow gives the limit
     if (cap > 0.0f) {
         const float a = 2.0f * LOG2E / cap;
+        const bool large = cap > 64.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = cap - 2.0f * cap * __fdividef(1.0f, exp2_approx(v[i] * a) + 1.0f);
+        for (int i = 0; i < N; ++i) {
+            const float z = v[i];
+            v[i] = fmaf(-2.0f * cap, __fdividef(1.0f, exp2_approx(z * a) + 1.0f), cap);
+            if (large) {
+                const float y = z / cap, y2 = y * y;
+                const float series =
+                    fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+                if (fabsf(y) < 0.25f) v[i] = z * series;
+            }
+        }
     }
 }
 
@@ -1487,6 +1499,9 @@ constexpr int LSE_SLICE = 8, LSE_SKINNY_SLICE = 2;
 constexpr int HEAD_SKINNY_ROWS = 64;
 constexpr int FP8_SKINNY_ROWS = 128;
 
+// Rows whose partial sums the workspace holds at once; more take several rounds.
+constexpr int LSE_ROWS = 16384;
+
 // Partial sums a row's logits come in.
 long long lse_parts(int N, int V, int num_sms) {
     return skinny_cols(N, HEAD_SKINNY_ROWS) ? 4ll * num_sms : 2 * ceil_div(V, TILE);
@@ -1546,7 +1561,8 @@ GradPlan grad_plan(int rows, int V, int D, int num_sms) {
 using namespace qs;
 
 extern "C" long long qs_head_loss_ws(int N, int V, int, int num_sms) {
-    return al(8ll * N * lse_parts(N, V, num_sms)) + al(4ll * N);
+    const long long rows = N < LSE_ROWS ? N : LSE_ROWS;
+    return al(8 * rows * lse_parts(N, V, num_sms)) + al(4 * rows);
 }
 
 extern "C" long long qs_head_grad_ws(int N, int V, int D, int num_sms) {
@@ -1554,7 +1570,8 @@ extern "C" long long qs_head_grad_ws(int N, int V, int D, int num_sms) {
     return g.dz_bytes + g.slab_bytes + g.rows_bytes;
 }
 
-extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream_t st) {
+// The loss of at most LSE_ROWS rows.
+static cudaError_t loss_round(const HeadCall* a, bool first, int* launches, cudaStream_t st) {
     float2* part = (float2*)a->ws;
     float* target_logit = (float*)(a->ws + al(8ll * a->N * lse_parts(a->N, a->V, a->num_sms)));
     int parts;
@@ -1574,7 +1591,7 @@ extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream
         p.part = part;
         p.target_logit = target_logit;
         parts = 4 * (a->num_sms < p.jobs ? a->num_sms : p.jobs);
-        e = launch_skinny<LSE>(cols, p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, true, st);
+        e = launch_skinny<LSE>(cols, p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, first, st);
     } else {
         Params p = {};
         e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
@@ -1593,12 +1610,27 @@ extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream
         p.part = part;
         p.target_logit = target_logit;
         parts = (int)ceil_div(a->V, 128);
-        e = launch<LSE>(p, a->num_sms, true, st);
+        e = launch<LSE>(p, a->num_sms, first, st);
     }
     if (e != cudaSuccess) return e;
-    *launches = 2;
+    *launches += 2;
     return launch_after(lse_join_kernel, ceil_div(a->N, 8), 1024, 0, st, (const float2*)part, (const float*)target_logit,
                         a->targets, a->N, a->V, parts, a->loss, a->lse_out);
+}
+
+extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream_t st) {
+    *launches = 0;
+    for (long long r = 0; r < a->N; r += LSE_ROWS) {
+        HeadCall part = *a;
+        part.hidden += r * a->hidden_stride;
+        part.targets += r;
+        part.loss += r;
+        part.lse_out += r;
+        part.N = (int)(a->N - r < LSE_ROWS ? a->N - r : LSE_ROWS);
+        const cudaError_t e = loss_round(&part, r == 0, launches, st);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream_t st) {

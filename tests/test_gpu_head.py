@@ -47,7 +47,7 @@ SIZES = [
 ]
 
 
-@pytest.mark.parametrize("cap", [0.0, 30.0, 2.0])
+@pytest.mark.parametrize("cap", [0.0, 30.0, 2.0, 1e5])
 @pytest.mark.parametrize("N,V,D", SIZES)
 def test_loss_and_gradients(torch, ctx, N, V, D, cap):
     h, w, t, g = H.head_inputs(N, V, D, seed=1, device="cuda")
@@ -77,6 +77,15 @@ def test_many_pieces_and_tiles(torch, ctx, N, V, D):
     # the bounds above add every rounding up; independent ones of half a bf16 step each stay far below
     assert (dh.double() - want["dh"]).norm() <= 2 * H.U16 * want["dh"].norm()
     assert (dw.double() - want["dw"]).norm() <= 2 * H.U16 * want["dw"].norm()
+
+
+def test_loss_of_many_rows(torch, ctx):
+    """More rows than one round of partial sums holds."""
+    h, w, t, _ = H.head_inputs(40000, 300, 64, seed=16, device="cuda")
+    want = H.head_exact(h, w, t, torch.ones(40000, device="cuda"), 0.0)
+    loss, lse = ctx.head_loss(h, w, t)
+    within(loss, want["loss"], want["eloss"], "loss")
+    within(lse, want["lse"], want["else"], "lse")
 
 
 def test_gradient_against_differences(torch, ctx):
@@ -485,7 +494,7 @@ def test_refusals(torch, ctx):
         ctx.head_loss(h, w, t[:4])
     with bad:
         ctx.head_loss(h.t(), w.t(), t)
-    for cap in (-1.0, float("nan"), float("inf")):
+    for cap in (-1.0, float("nan"), float("inf"), 1e-30, 1e30):
         with bad:
             ctx.head_loss(h, w, t, softcap=cap)
     with pytest.raises(qsamp.QsampError, match="multiple of 8") as e:
