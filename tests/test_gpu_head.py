@@ -44,6 +44,7 @@ def guarded(torch, rows, cols, pad, dtype):
 SIZES = [
     (1, 1, 8), (1, 2, 16), (1, 257, 64), (3, 31, 8), (5, 1000, 72), (33, 128, 40), (64, 255, 1024), (127, 256, 64),
     (130, 513, 128), (257, 4099, 264), (300, 1025, 200), (512, 300, 520), (17, 20011, 96), (700, 70, 48),
+    (16, 400, 64), (32, 400, 64), (65, 400, 64), (129, 20011, 64),
 ]
 
 
@@ -338,7 +339,9 @@ def test_quantiser_many_rows(torch, ctx):
 # ---------------------------------------------------------------- 8-bit product
 @pytest.mark.parametrize("f32", [False, True])
 @pytest.mark.parametrize("M,V,K", [(1, 1, 1), (1, 129, 128), (2, 300, 16), (10, 1001, 400), (33, 255, 127), (128, 128, 256),
-                                   (129, 4097, 513), (256, 512, 1024), (300, 700, 1000), (1000, 130, 2056)])
+                                   (129, 4097, 513), (256, 512, 1024), (300, 700, 1000), (1000, 130, 2056),
+                                   (16, 300, 260), (17, 300, 260), (64, 300, 260), (65, 300, 260), (20, 30011, 300),
+                                   (600, 20011, 2100), (100, 300, 8320), (5, 200, 66000)])
 def test_product(torch, ctx, M, V, K, f32):
     x, sx, w, sw = H.fp8_inputs(M, V, K, device="cuda")
     kp = -(-K // 16) * 16
@@ -380,6 +383,67 @@ def test_product_strided_scales(torch, ctx):
     bw = torch.full((3, 5), float("nan"), device="cuda")
     bx[:, 1:4], bw[:, 2:5] = sx, sw
     assert torch.equal(out, ctx.matmul_fp8(x, bx[:, 1:4], w, bw[:, 2:5]))
+
+
+# ---------------------------------------------------------------- far offsets
+def roomy(torch, gib):
+    if torch.cuda.mem_get_info()[0] < gib * 2**30:
+        pytest.skip(f"needs {gib} GB")
+
+
+def test_offsets_past_32_bits_product(torch, ctx):
+    """A result of more than 2^31 elements: its last rows are those of a small call."""
+    roomy(torch, 30)
+    M, V, K = 8300, 262144, 128
+    x, sx, w, sw = H.fp8_inputs(300, V, K, seed=5, device="cuda")
+    big = torch.zeros((M, K), dtype=torch.uint8, device="cuda").view(x.dtype)
+    bs = torch.zeros((M, 1), device="cuda")
+    big[-300:] = x
+    bs[-300:] = sx
+    out = ctx.matmul_fp8(big, bs, w, sw)
+    assert out.numel() > 2**31
+    assert torch.equal(out[-300:], ctx.matmul_fp8(x, sx, w, sw)) and (out[:256] == 0).all()
+
+
+def test_offsets_past_32_bits_quantiser(torch, ctx):
+    roomy(torch, 30)
+    M, K = 263000, 8192
+    x = torch.randn((M, 64), device="cuda").to(torch.bfloat16).repeat(1, K // 64)
+    assert x.numel() > 2**31
+    for rows in (1, 128):
+        q, s = ctx.quantize_fp8(x, block_rows=rows)
+        tail = M // 128 * 128 - 256
+        q2, s2 = ctx.quantize_fp8(x[tail:], block_rows=rows)
+        assert torch.equal(q[tail:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s[tail // rows:], s2)
+        del q, s
+
+
+def test_offsets_past_32_bits_gradients(torch, ctx):
+    """A weight of more than 2^31 elements: loss and the gradients of its last
+    rows (one of them a target), and of the hidden rows."""
+    roomy(torch, 60)
+    N, V, D = 3, 262200, 8200
+    g = torch.Generator(device="cuda").manual_seed(6)
+    w = torch.empty((V, D), dtype=torch.bfloat16, device="cuda")
+    for r in range(0, V, 30000):
+        w[r:r + 30000] = torch.randn((min(30000, V - r), D), generator=g, device="cuda") * (2.0 / D**0.5)
+    h = torch.randn((N, D), generator=g, device="cuda").to(torch.bfloat16)
+    t = torch.tensor([V - 1, 5, V - 200], dtype=torch.int32, device="cuda")
+    z = torch.cat([h.double() @ w[r:r + 30000].double().t() for r in range(0, V, 30000)], dim=1)
+    lse64 = torch.logsumexp(z, dim=1)
+    loss, lse = ctx.head_loss(h, w, t)
+    err = (D + 8) * H.U32 * (h.double().abs() @ w[-1000:].double().abs().t()).max() * 2 + (V + 256) * H.U32
+    assert (lse - lse64).abs().max() <= err + 4 * H.U32 * lse64.max()
+    assert (loss - (lse64 - z.gather(1, t.long()[:, None])[:, 0])).abs().max() <= 2 * err + 8 * H.U32 * lse64.max()
+    grad = torch.tensor([1.0, -0.5, 0.25], device="cuda")
+    dh, dw = ctx.head_loss_grad(h, w, t, lse, grad)
+    p = torch.exp(z - lse64[:, None])
+    p[torch.arange(N), t.long()] -= 1
+    dz = p * grad.double()[:, None]
+    want = dz[:, -300:].t() @ h.double()
+    assert (dw[-300:].double() - want).norm() <= 1.01 * H.U16 * want.norm()
+    want = sum(dz[:, r:r + 30000] @ w[r:r + 30000].double() for r in range(0, V, 30000))
+    assert (dh.double() - want).norm() <= 1.01 * H.U16 * want.norm()
 
 
 # ---------------------------------------------------------------- together
