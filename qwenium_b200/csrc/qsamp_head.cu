@@ -808,8 +808,9 @@ struct SkinnyControl {
 static_assert(sizeof(SkinnyControl) <= 512, "control block");
 
 struct SkinnyParams {
-    CUtensorMap a, b;  // weight (128 rows a box) and hidden rows (COLS a box)
+    CUtensorMap a, b;  // weight (a tile's rows a box) and hidden rows (COLS a box)
     int V, M, k_blocks, slice, jobs;
+    int tile;          // weight rows of a tile: at most 128, so that every CTA has the same number of tiles
     int* status;
     const int32_t* targets;
     float softcap;
@@ -877,22 +878,6 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
         tma_prefetch_map(&p.b);
     }
     if (warp == 1) tmem_alloc<false>(smem_addr(&ctl.tmem), 512);
-    launch_next();
-    wait_previous();
-    if (MODE == DZ && threadIdx.x < COLS) {
-        const int i = threadIdx.x, t = i < p.M ? p.targets[i] : -1;
-        const bool has = t >= 0 && t < p.V_total;
-        table[i] = has ? p.lse[i] : 0.0f;
-        table[COLS + i] = has ? p.grad[i] : 0.0f;
-        ((int*)table)[2 * COLS + i] = has ? t - p.n0 : INT32_MIN;
-    }
-    if (MODE == FP8) {
-        // the rows' scales, K block by K block: every lane reads the same four at a time
-        for (int i = threadIdx.x; i < p.k_blocks * COLS; i += S::THREADS) {
-            const int m = i % COLS;
-            table[i] = m < p.M ? p.sx[m * p.sx_stride + i / COLS] : 0.0f;
-        }
-    }
     fence_before();
     __syncthreads();
     fence_after();
@@ -900,7 +885,8 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
     volatile int* gave_up = &ctl.gave_up;
     const uint32_t full0 = smem_addr(ctl.full), empty0 = smem_addr(ctl.empty);
     const uint32_t acc_full0 = smem_addr(ctl.acc_full), acc_empty0 = smem_addr(ctl.acc_empty);
-
+    launch_next();
+    wait_previous();
     if (warp == 0) {
         Ring<S::DEPTH> at;
         bool ok = true;
@@ -909,9 +895,9 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
                 if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status))) break;
                 if (elected()) {
                     const uint32_t full = full0 + 8 * at.slot, da = stage0 + at.slot * S::STAGE;
-                    bar_expect(full, S::STAGE);
+                    bar_expect(full, p.tile * 128 + S::B_BYTES);
                     const int x = kb * (MODE == FP8 ? 128 : 64);
-                    tma_load<false>(da, &p.a, x, job * 128, full);
+                    tma_load<false>(da, &p.a, x, job * p.tile, full);
                     tma_load<false>(da + S::A_BYTES, &p.b, x, 0, full);
                 }
                 __syncwarp();
@@ -957,6 +943,23 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
         }
     } else {
         const int quarter = warp % 4, c0 = (warp - 2) / 4 * PART, mine = p.M - c0;  // rows from c0
+        // what the epilogue needs of the rows; the loads are under way meanwhile
+        const int thread = threadIdx.x - 64;
+        if (MODE == DZ && thread < COLS) {
+            const int t = thread < p.M ? p.targets[thread] : -1;
+            const bool has = t >= 0 && t < p.V_total;
+            table[thread] = has ? p.lse[thread] : 0.0f;
+            table[COLS + thread] = has ? p.grad[thread] : 0.0f;
+            ((int*)table)[2 * COLS + thread] = has ? t - p.n0 : INT32_MIN;
+        }
+        if (MODE == FP8) {
+            // the rows' scales, K block by K block: every lane reads the same four at a time
+            for (int i = thread; i < p.k_blocks * COLS; i += 32 * S::EPI) {
+                const int m = i % COLS;
+                table[i] = m < p.M ? p.sx[m * p.sx_stride + i / COLS] : 0.0f;
+            }
+        }
+        if (MODE != LSE) asm volatile("bar.sync 1, %0;" ::"n"(32 * S::EPI) : "memory");
         const uint32_t base = tmem + (quarter << 21) + c0;
         const int slices = (p.k_blocks + p.slice - 1) / p.slice;
         Ring<S::BUFS> acc;
@@ -966,16 +969,24 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
 #pragma unroll
         for (int i = 0; i < (MODE == LSE ? PART : 1); ++i) mx[i] = -3.402823466e38f, se[i] = 0.0f;
         for (int job = blockIdx.x; ok && job < p.jobs; job += gridDim.x) {
-            const int v0 = job * 128 + quarter * 32, v = v0 + lane;
-            const float* sw = MODE == FP8 ? p.sw + job * p.sw_stride : nullptr;
-            float sum[PART], w32 = 0.0f;  // FP8: the weight block's scales, 32 K blocks in the lanes
+            const int v = job * p.tile + quarter * 32 + lane;
+            const bool live = quarter * 32 + lane < p.tile && v < p.V;
+            // FP8: scales of the one or two blocks of weight rows the tile lies in, 32 K blocks in the lanes
+            const int block0 = job * p.tile / FP8_BLOCK, block1 = min(block0 + 1, (p.V - 1) / FP8_BLOCK);
+            const bool second = v / FP8_BLOCK > block0;
+            float sum[PART], w32 = 0.0f, w32b = 0.0f;
 #pragma unroll
             for (int i = 0; i < PART; ++i) sum[i] = 0.0f;
             for (int kb = 0; kb < slices; ++kb, acc.step()) {
                 float now = 1.0f;
                 if (MODE == FP8) {
-                    if (kb % 32 == 0) w32 = sw[min(kb + lane, slices - 1)];
-                    now = __shfl_sync(0xffffffffu, w32, kb % 32);
+                    if (kb % 32 == 0) {
+                        const int at = min(kb + lane, slices - 1);
+                        w32 = p.sw[block0 * p.sw_stride + at];
+                        w32b = p.sw[block1 * p.sw_stride + at];
+                    }
+                    const float a = __shfl_sync(0xffffffffu, w32, kb % 32), b = __shfl_sync(0xffffffffu, w32b, kb % 32);
+                    now = second ? b : a;
                 }
                 ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                 if (!ok) break;
@@ -985,7 +996,7 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
                 __syncwarp();
                 if (lane == 0) bar_arrive(acc_empty0 + 8 * acc.slot);
             }
-            if (!ok || v >= p.V) continue;
+            if (!ok || !live) continue;
             if constexpr (MODE == LSE) {
 #pragma unroll
                 for (int c = 0; c < PART; c += 16) logits_of(reinterpret_cast<float(&)[16]>(sum[c]), p.softcap);
@@ -1463,10 +1474,15 @@ int skinny_cols(int rows, int most) {
 }
 
 template <int MODE, int COLS>
-cudaError_t launch_skinny(SkinnyParams& p, const void* hidden, int esz, long long cols, long long stride, int num_sms, bool first,
-                          cudaStream_t st) {
+cudaError_t launch_skinny(SkinnyParams& p, const void* weight, long long weight_stride, const void* hidden, int esz, long long cols,
+                          long long stride, int num_sms, bool first, cudaStream_t st) {
     using S = Skinny<MODE, COLS>;
-    cudaError_t e = make_map(&p.b, hidden, esz, p.M, cols, stride, COLS);
+    // as few tiles a CTA as 128 rows allow, of as few rows as that number allows
+    const long long most = ceil_div(p.V, 128ll * num_sms) * num_sms;
+    p.tile = (int)ceil_div(p.V, most);
+    p.jobs = (int)ceil_div(p.V, p.tile);
+    cudaError_t e = make_map(&p.a, weight, esz, p.V, cols, weight_stride, p.tile);
+    if (e == cudaSuccess) e = make_map(&p.b, hidden, esz, p.M, cols, stride, COLS);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(skinny_kernel<MODE, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return e;
     const int blocks = num_sms < p.jobs ? num_sms : p.jobs;
@@ -1475,14 +1491,14 @@ cudaError_t launch_skinny(SkinnyParams& p, const void* hidden, int esz, long lon
     return cudaGetLastError();
 }
 template <int MODE>
-cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* hidden, int esz, long long width, long long stride, int num_sms,
-                          bool first, cudaStream_t st) {
-    if (cols == 16) return launch_skinny<MODE, 16>(p, hidden, esz, width, stride, num_sms, first, st);
-    if (cols == 32) return launch_skinny<MODE, 32>(p, hidden, esz, width, stride, num_sms, first, st);
+cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* weight, long long weight_stride, const void* hidden, int esz,
+                          long long width, long long stride, int num_sms, bool first, cudaStream_t st) {
+    if (cols == 16) return launch_skinny<MODE, 16>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, first, st);
+    if (cols == 32) return launch_skinny<MODE, 32>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, first, st);
     if constexpr (MODE == FP8) {
-        if (cols == 128) return launch_skinny<MODE, 128>(p, hidden, esz, width, stride, num_sms, first, st);
+        if (cols == 128) return launch_skinny<MODE, 128>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, first, st);
     }
-    return launch_skinny<MODE, 64>(p, hidden, esz, width, stride, num_sms, first, st);
+    return launch_skinny<MODE, 64>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, first, st);
 }
 
 // K blocks of 64 whose products are summed in tensor memory before fp32
@@ -1578,20 +1594,17 @@ static cudaError_t loss_round(const HeadCall* a, bool first, int* launches, cuda
     cudaError_t e;
     if (const int cols = skinny_cols(a->N, HEAD_SKINNY_ROWS)) {
         SkinnyParams p = {};
-        e = make_map(&p.a, a->weight, 2, a->V, a->D, a->weight_stride, 128);
-        if (e != cudaSuccess) return e;
         p.V = a->V;
         p.M = a->N;
         p.k_blocks = (int)ceil_div(a->D, 64);
         p.slice = LSE_SKINNY_SLICE;
-        p.jobs = (int)ceil_div(a->V, 128);
         p.status = a->status;
         p.targets = a->targets;
         p.softcap = a->softcap;
         p.part = part;
         p.target_logit = target_logit;
+        e = launch_skinny<LSE>(cols, p, a->weight, a->weight_stride, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, first, st);
         parts = 4 * (a->num_sms < p.jobs ? a->num_sms : p.jobs);
-        e = launch_skinny<LSE>(cols, p, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, first, st);
     } else {
         Params p = {};
         e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
@@ -1660,15 +1673,12 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.status = a->status;
         if (cols) {
             SkinnyParams f = {};
-            e = make_map(&f.a, weight, 2, pw, a->D, a->weight_stride, 128);
-            if (e != cudaSuccess) return e;
             f.V = pw;
             f.V_total = a->V;
             f.n0 = p0;
             f.M = a->N;
             f.k_blocks = (int)ceil_div(a->D, 64);
             f.slice = f.k_blocks;
-            f.jobs = (int)ceil_div(pw, 128);
             f.status = a->status;
             f.targets = a->targets;
             f.softcap = a->softcap;
@@ -1676,7 +1686,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             f.grad = a->grad_loss;
             f.dz = dz;
             f.dz_pitch = g.piece;
-            e = launch_skinny<DZ>(cols, f, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, false, st);
+            e = launch_skinny<DZ>(cols, f, weight, a->weight_stride, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, false, st);
         } else {
             e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
             if (e == cudaSuccess) e = make_map(&p.b, weight, 2, pw, a->D, a->weight_stride, 128);
@@ -1727,13 +1737,10 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
     const long long blocks = ceil_div(a->K, FP8_BLOCK);
     if (cols && blocks * cols * 4 <= Skinny<FP8, 16>::TABLE) {
         SkinnyParams p = {};
-        const cudaError_t e = make_map(&p.a, a->w, 1, a->V, a->K, a->w_stride, 128);
-        if (e != cudaSuccess) return e;
         p.V = a->V;
         p.M = a->M;
         p.k_blocks = (int)blocks;
         p.slice = 1;
-        p.jobs = (int)ceil_div(a->V, 128);
         p.status = a->status;
         p.sx = a->sx;
         p.sw = a->sw;
@@ -1742,7 +1749,7 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
         p.out = a->out;
         p.out_stride = a->out_stride;
         p.out_bf16 = a->out_bf16;
-        return launch_skinny<FP8>(cols, p, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
+        return launch_skinny<FP8>(cols, p, a->w, a->w_stride, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
     }
     WideParams p = {};
     cudaError_t e = make_map(&p.a, a->x, 1, a->M, a->K, a->x_stride, 128);
