@@ -116,6 +116,7 @@ struct qsamp_ctx {
     // out (they have no per-call status to clear or copy); read and cleared by
     // qsamp_poll_status
     int* head_status = nullptr;
+    uint32_t head_ready = 0;  // output-head kernels whose attributes are set on this device
     // device-side bounds (qsamp_set_limits)
     int max_rounds = kMaxRounds;
     unsigned long long ready_wait_ns = 1000000000ull;
@@ -1389,6 +1390,7 @@ static qsamp_status head_call(qsamp_ctx* c, const qsamp_head* h, int grad, void*
     a.ws = (unsigned char*)workspace;
     a.num_sms = c->num_sms;
     a.status = c->head_status;
+    a.ready = &c->head_ready;
     return QSAMP_OK;
 }
 
@@ -1511,6 +1513,7 @@ qsamp_status qsamp_matmul_fp8(qsamp_ctx* c, const qsamp_fp8_product* p, void* st
     a.out_stride = p->out_stride;
     a.num_sms = c->num_sms;
     a.status = c->head_status;
+    a.ready = &c->head_ready;
     return on_device(c, "8-bit product launch", [&](int* n) {
         *n = 1;
         return qs_matmul_fp8(&a, (cudaStream_t)stream);

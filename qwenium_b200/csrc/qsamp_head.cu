@@ -11,6 +11,12 @@
 // on the accumulators: a thread owns one row (lane) and 128 columns (half).
 // The pair halves what each SM loads per flop: 32 KB per 512 tensor cycles
 // instead of 48 KB, which the L2 could not feed to 148 SMs.
+//
+// Measured (4096 x 2048 x 151936, one launch at full clock): loss 1.57 ms = 1.62
+// PFLOP/s, dz of five pieces 1.55 ms, gradients 3.2 ms = 1.58 PFLOP/s; the
+// tensor pipe is 74 to 78% active. In a loop the 1000 W limit sets the pace
+// (8.0 ms a step, 1.17 GHz): 91% of cuBLAS's sustained rate over the 8 N D V
+// operations, a quarter of them the logits made a second time.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -494,12 +500,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
 // ---------------------------------------------------------------- 8-bit product
 // The block-scaled product of many rows. Scales differ from K block to K
 // block, so each block's sums leave tensor memory after four instructions and
-// are added up in registers: a round trip per 512 tensor cycles, which sets
-// the pace. What shortens it: sixteen epilogue warps of 64 columns each (two
-// loads and 32 packed fmas a block), accumulators handed over in halves of
-// 128 columns, so that one half is read while the other is filled, and
-// scales brought to shared memory by asynchronous copies 16 K blocks ahead
-// (read from global memory they cost 800 cycles a block).
+// are added up in registers: a round trip (instructions, signal, read, signal
+// back) per two blocks, which sets the pace with the power limit. What shortens
+// it: sixteen epilogue warps of 64 columns each (four loads and 32 packed fmas
+// a block), accumulators handed over in halves of 128 columns, so that one
+// half is read while the other is filled, and scales brought to shared memory
+// by asynchronous copies 16 K blocks ahead (read from global memory they cost
+// 800 cycles a block). Measured: 256 x 4096 x 151936 in 223 us (tensor pipe 36%
+// active, 1.00x of the bytes), 255 in a loop at 1.58 GHz; 4096 x 4048 x 16384 in
+// 350 us = 1.55 PFLOP/s.
 constexpr int WIDE_EPI = 16;
 constexpr int WIDE_THREADS = 32 * (2 + WIDE_EPI);
 constexpr int CHUNK = 16;   // K blocks of scales copied at once
@@ -790,6 +799,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
 // the matrix instructions cost COLS columns instead of 256, and tensor memory
 // holds 512 / COLS accumulators (up to eight are used), which hides the
 // epilogue's round trip behind the weight's loads. Every CTA works alone.
+// Measured: 8-bit, 1 x 4096 x 151936 in 105 us = 5.9 TB/s (91% of the copy rate),
+// loss of 1 x 2048 x 151936 in 102 us = 6.1 TB/s with its join.
 template <int MODE, int COLS>
 struct Skinny {
     static constexpr int PART = COLS < 32 ? COLS : 32;  // columns of an epilogue warp: four warps for each 32
@@ -1288,8 +1299,9 @@ __device__ __forceinline__ void store8(uint8_t* row, int k, int K, bool vec, uin
 // Blocks of one row: eight threads a block, sixteen values a thread (two
 // pieces, so that a load's lanes are neighbours); a warp takes 512 columns of
 // four rows with all their loads in flight. Each value is read once and held
-// in registers between the maximum and the quotients. FULL: whole blocks and
-// whole groups of rows on aligned addresses, without checks per value (which
+// in registers between the maximum and the quotients (8000 x 8192 bf16 in 38
+// us = 5.1 TB/s, its instructions' rate; the square blocks' kernel 151936 x
+// 4096 in 277 us = 6.7 TB/s). FULL: whole blocks and whole groups of rows on aligned addresses, without checks per value (which
 // would cost registers, and a quarter of the rate). A CTA's warps lie below
 // each other, so that the few slower ones at the right edge share CTAs.
 constexpr int QROWS = 4, QCOLS = 512;
@@ -1437,6 +1449,21 @@ cudaError_t make_map(CUtensorMap* map, const void* base, int esz, long long rows
                : cudaErrorInvalidValue;
 }
 
+// Lets a kernel use its dynamic shared memory, once per context: `bit` is the
+// kernel's in *ready.
+template <typename K>
+cudaError_t allow_smem(K* kernel, int bytes, int bit, uint32_t* ready) {
+    if (*ready >> bit & 1) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) *ready |= 1u << bit;
+    return e;
+}
+// Bits: the pair kernel's modes 0 to 2, the wide kernel 3, the few-row kernel's
+// modes times column counts from 4.
+constexpr int WIDE_BIT = 3;
+constexpr int skinny_bit(int mode, int cols) { return 4 + mode * 4 + (cols == 16 ? 0 : cols == 32 ? 1 : cols == 64 ? 2 : 3); }
+static_assert(skinny_bit(FP8, 128) < 32, "bits of a word");
+
 // A launch that may begin before the call's previous kernel has ended (the
 // kernel calls wait_previous).
 template <typename... A, typename... B>
@@ -1455,11 +1482,11 @@ cudaError_t launch_after(void (*kernel)(A...), long long blocks, int threads, in
 }
 
 template <int MODE>
-cudaError_t launch(const Params& p, int num_sms, bool first, cudaStream_t st) {
+cudaError_t launch(const Params& p, const HeadCall* a, bool first, cudaStream_t st) {
     constexpr int smem = smem_bytes(MODE);
-    cudaError_t e = cudaFuncSetAttribute(head_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = allow_smem(head_kernel<MODE>, smem, MODE, a->ready);
     if (e != cudaSuccess) return e;
-    const int pairs = num_sms / 2 < p.jobs ? num_sms / 2 : p.jobs;
+    const int pairs = a->num_sms / 2 < p.jobs ? a->num_sms / 2 : p.jobs;
     if (!first) return launch_after(head_kernel<MODE>, 2 * pairs, THREADS, smem, st, p);
     head_kernel<MODE><<<2 * pairs, THREADS, smem, st>>>(p);
     return cudaGetLastError();
@@ -1475,7 +1502,7 @@ int skinny_cols(int rows, int most) {
 
 template <int MODE, int COLS>
 cudaError_t launch_skinny(SkinnyParams& p, const void* weight, long long weight_stride, const void* hidden, int esz, long long cols,
-                          long long stride, int num_sms, bool first, cudaStream_t st) {
+                          long long stride, int num_sms, uint32_t* ready, bool first, cudaStream_t st) {
     using S = Skinny<MODE, COLS>;
     // as few tiles a CTA as 128 rows allow, of as few rows as that number allows
     const long long most = ceil_div(p.V, 128ll * num_sms) * num_sms;
@@ -1483,7 +1510,7 @@ cudaError_t launch_skinny(SkinnyParams& p, const void* weight, long long weight_
     p.jobs = (int)ceil_div(p.V, p.tile);
     cudaError_t e = make_map(&p.a, weight, esz, p.V, cols, weight_stride, p.tile);
     if (e == cudaSuccess) e = make_map(&p.b, hidden, esz, p.M, cols, stride, COLS);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(skinny_kernel<MODE, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e == cudaSuccess) e = allow_smem(skinny_kernel<MODE, COLS>, S::SMEM, skinny_bit(MODE, COLS), ready);
     if (e != cudaSuccess) return e;
     const int blocks = num_sms < p.jobs ? num_sms : p.jobs;
     if (!first) return launch_after(skinny_kernel<MODE, COLS>, blocks, S::THREADS, S::SMEM, st, p);
@@ -1492,13 +1519,13 @@ cudaError_t launch_skinny(SkinnyParams& p, const void* weight, long long weight_
 }
 template <int MODE>
 cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* weight, long long weight_stride, const void* hidden, int esz,
-                          long long width, long long stride, int num_sms, bool first, cudaStream_t st) {
-    if (cols == 16) return launch_skinny<MODE, 16>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, first, st);
-    if (cols == 32) return launch_skinny<MODE, 32>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, first, st);
+                          long long width, long long stride, int num_sms, uint32_t* ready, bool first, cudaStream_t st) {
+    if (cols == 16) return launch_skinny<MODE, 16>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, ready, first, st);
+    if (cols == 32) return launch_skinny<MODE, 32>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, ready, first, st);
     if constexpr (MODE == FP8) {
-        if (cols == 128) return launch_skinny<MODE, 128>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, first, st);
+        if (cols == 128) return launch_skinny<MODE, 128>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, ready, first, st);
     }
-    return launch_skinny<MODE, 64>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, first, st);
+    return launch_skinny<MODE, 64>(p, weight, weight_stride, hidden, esz, width, stride, num_sms, ready, first, st);
 }
 
 // K blocks of 64 whose products are summed in tensor memory before fp32
@@ -1509,9 +1536,9 @@ cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* weight, long lo
 // 13% at 4.
 constexpr int LSE_SLICE = 8, LSE_SKINNY_SLICE = 2;
 // Measured on both sides (V 151936; few-row kernel against the pair's, us):
-// loss, D 2048: 1 row 104 / 149, 32 rows 113 / 123, 64 rows 115 / 124, 128
-// rows 156 / 129. 8-bit product, K 4096: 1 row 110 / 197, 64 rows 148 / 189,
-// 128 rows 201 / 202 (V 32000, K 2048: 32 / 35), 256 rows 348 / 212.
+// loss, D 2048: 1 row 102 / 149, 32 rows 110 / 123, 64 rows 118 / 124, 128
+// rows 156 / 126. 8-bit product, K 4096: 1 row 106 / 197, 64 rows 143 / 189,
+// 128 rows 180 / 202; 256 rows in two groups 348 / 212.
 constexpr int HEAD_SKINNY_ROWS = 64;
 constexpr int FP8_SKINNY_ROWS = 128;
 
@@ -1603,7 +1630,7 @@ static cudaError_t loss_round(const HeadCall* a, bool first, int* launches, cuda
         p.softcap = a->softcap;
         p.part = part;
         p.target_logit = target_logit;
-        e = launch_skinny<LSE>(cols, p, a->weight, a->weight_stride, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, first, st);
+        e = launch_skinny<LSE>(cols, p, a->weight, a->weight_stride, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, a->ready, first, st);
         parts = 4 * (a->num_sms < p.jobs ? a->num_sms : p.jobs);
     } else {
         Params p = {};
@@ -1623,7 +1650,7 @@ static cudaError_t loss_round(const HeadCall* a, bool first, int* launches, cuda
         p.part = part;
         p.target_logit = target_logit;
         parts = (int)ceil_div(a->V, 128);
-        e = launch<LSE>(p, a->num_sms, first, st);
+        e = launch<LSE>(p, a, first, st);
     }
     if (e != cudaSuccess) return e;
     *launches += 2;
@@ -1686,7 +1713,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             f.grad = a->grad_loss;
             f.dz = dz;
             f.dz_pitch = g.piece;
-            e = launch_skinny<DZ>(cols, f, weight, a->weight_stride, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, false, st);
+            e = launch_skinny<DZ>(cols, f, weight, a->weight_stride, a->hidden, 2, a->D, a->hidden_stride, a->num_sms, a->ready, false, st);
         } else {
             e = make_map(&p.a, a->hidden, 2, a->N, a->D, a->hidden_stride, 128);
             if (e == cudaSuccess) e = make_map(&p.b, weight, 2, pw, a->D, a->weight_stride, 128);
@@ -1700,7 +1727,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             p.softcap = a->softcap;
             p.lse = a->lse;
             p.grad = a->grad_loss;
-            e = launch<DZ>(p, a->num_sms, false, st);
+            e = launch<DZ>(p, a, false, st);
         }
         if (e != cudaSuccess) return e;
         p.m_tiles = (int)ceil_div(R, TILE);
@@ -1723,7 +1750,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.D = a->D;
         p.slabs = slabs;
         p.add = q > 0;
-        e = launch<GRAD>(p, a->num_sms, false, st);
+        e = launch<GRAD>(p, a, false, st);
         if (e != cudaSuccess) return e;
         *launches += 2;
     }
@@ -1749,12 +1776,12 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
         p.out = a->out;
         p.out_stride = a->out_stride;
         p.out_bf16 = a->out_bf16;
-        return launch_skinny<FP8>(cols, p, a->w, a->w_stride, a->x, 1, a->K, a->x_stride, a->num_sms, true, st);
+        return launch_skinny<FP8>(cols, p, a->w, a->w_stride, a->x, 1, a->K, a->x_stride, a->num_sms, a->ready, true, st);
     }
     WideParams p = {};
     cudaError_t e = make_map(&p.a, a->x, 1, a->M, a->K, a->x_stride, 128);
     if (e == cudaSuccess) e = make_map(&p.b, a->w, 1, a->V, a->K, a->w_stride, 128);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WIDE_SMEM);
+    if (e == cudaSuccess) e = allow_smem(wide_kernel, WIDE_SMEM, WIDE_BIT, a->ready);
     if (e != cudaSuccess) return e;
     p.m_tiles = (int)ceil_div(a->M, TILE);
     p.n_tiles = (int)ceil_div(a->V, TILE);

@@ -30,7 +30,8 @@ struct HeadCall {
     long long d_hidden_stride, d_weight_stride;
     unsigned char* ws;
     int num_sms;
-    int* status;  // mapped host word, written only when a bounded wait ran out
+    int* status;      // mapped host word, written only when a bounded wait ran out
+    uint32_t* ready;  // the context's kernels whose attributes are set
 };
 
 // One 8-bit product: out[m][n] = sum over K blocks of sx sw (x . w).
@@ -44,6 +45,7 @@ struct Fp8Call {
     long long x_stride, w_stride, sx_stride, sw_stride, out_stride;
     int num_sms;
     int* status;
+    uint32_t* ready;
 };
 
 constexpr int FP8_BLOCK = 128;

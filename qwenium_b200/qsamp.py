@@ -619,14 +619,14 @@ class Context:
         return torch.cuda.current_stream(self._torch_device()).cuda_stream if stream is None else int(stream)
 
     def _tensor(self, name, t, dtypes, shape):
-        """Checks a CUDA tensor argument: its dtype, its shape (None: any
-        size), this context's device, unit stride in the last dimension."""
-        if not t.is_cuda or t.get_device() != self.device:
-            raise QsampError(1, f"{name}: expected a tensor on cuda:{self.device}, got {t.device}")
+        """Checks a CUDA tensor argument: its dtype, its shape (one or two
+        sizes, None: any), this context's device, unit stride in the last dimension."""
         if t.dtype not in dtypes:
             raise QsampError(1, f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
+        if t.get_device() != self.device or not t.is_cuda:
+            raise QsampError(1, f"{name}: expected a tensor on cuda:{self.device}, got {t.device}")
         got = t.shape
-        if len(got) != len(shape) or any(w is not None and w != g for w, g in zip(shape, got)):
+        if len(got) != len(shape) or got[0] != shape[0] and shape[0] is not None or got[-1] != shape[-1] and shape[-1] is not None:
             raise QsampError(1, f"{name}: expected shape {tuple(shape)}, got {tuple(got)}")
         if got[-1] > 1 and t.stride(-1) != 1:
             raise QsampError(1, f"{name}: expected unit stride in the last dimension, got {t.stride()}")
