@@ -148,20 +148,20 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
 // at a cap of 30 the plain form is within 1e-5).
 template <int N>
 __device__ __forceinline__ void logits_of(float (&v)[N], float cap) {
-    if (cap > 0.0f) {
-        const float a = 2.0f * LOG2E / cap;
-        const bool large = cap > 64.0f;
+    if (cap == 0.0f) return;
+    const float a = 2.0f * LOG2E / cap, b = -2.0f * cap;
+    if (cap <= 64.0f) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float z = v[i];
-            v[i] = fmaf(-2.0f * cap, __fdividef(1.0f, exp2_approx(z * a) + 1.0f), cap);
-            if (large) {
-                const float y = z / cap, y2 = y * y;
-                const float series =
-                    fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-                if (fabsf(y) < 0.25f) v[i] = z * series;
-            }
-        }
+        for (int i = 0; i < N; ++i) v[i] = fmaf(b, __fdividef(1.0f, exp2_approx(v[i] * a) + 1.0f), cap);
+        return;
+    }
+    const float inv = 1.0f / cap;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float y = v[i] * inv, y2 = y * y;
+        const float series = fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+        const float whole = fmaf(b, __fdividef(1.0f, exp2_approx(v[i] * a) + 1.0f), cap);
+        v[i] = fabsf(y) < 0.25f ? v[i] * series : whole;
     }
 }
 
