@@ -227,9 +227,10 @@ template <int MODE>
 struct Epilogue;
 
 // dz = g (exp(l - lse) - [target]) (1 - (l / cap)^2); 0 for rows without a
-// gradient.
+// gradient. Without a cap (inv_cap 0) the slope is 1 for a logit of -infinity
+// too: y is 0 times the lowest finite number there.
 __device__ __forceinline__ float dz_of(float l, float lse, float g, float inv_cap, bool hot, bool none) {
-    const float y = l * inv_cap, d = exp2_approx((l - lse) * LOG2E) - (hot ? 1.0f : 0.0f);
+    const float y = fmaxf(l, -3.402823466e38f) * inv_cap, d = exp2_approx((l - lse) * LOG2E) - (hot ? 1.0f : 0.0f);
     return none ? 0.0f : d * fmaf(-y, y, 1.0f) * g;
 }
 

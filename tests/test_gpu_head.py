@@ -201,6 +201,34 @@ def test_a_bad_row_stays_alone(torch, ctx):
     assert torch.equal(loss[ok], loss0[ok]) and torch.equal(lse[ok], lse0[ok]) and torch.equal(dh[ok], dh0[ok])
 
 
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("N", [20, 150])
+def test_logits_of_minus_infinity(torch, ctx, N, cap):
+    """Finite factors whose product passes fp32's range, as the first and the
+    last token's logit of each row: without a soft-cap these tokens take no part
+    and have no gradient, as though they were not there; with one their logit is -cap."""
+    V, D = 400, 64
+    h, w, t, g = H.head_inputs(N, V, D, seed=16, device="cuda")
+    h[:, 0] = 4.0
+    w[:, 0] = 0.0
+    low = torch.zeros((1, D), dtype=torch.bfloat16, device="cuda")
+    low[0, 0] = -(2.0**127)
+    wide = torch.cat([low, w, low])
+    at = torch.where(t >= 0, t + 1, t)
+    loss, lse = ctx.head_loss(h, wide, at, softcap=cap)
+    dh, dw = ctx.head_loss_grad(h, wide, at, lse, g, softcap=cap)
+    assert torch.isfinite(loss).all() and torch.isfinite(lse).all()
+    # dz of the two tokens is exactly 0: exp(-inf), or a slope 1 - (l / cap)^2 of at most a rounding, times -2^127
+    assert torch.isfinite(dh[:, 1:]).all() and torch.isfinite(dw[1:-1]).all()
+    if cap == 0.0:
+        assert (dw[0] == 0).all() and (dw[-1] == 0).all()
+        want = H.head_exact(h, w, t, g, 0.0)
+        within(loss, want["loss"], want["eloss"], "loss")
+        within(lse, want["lse"], want["else"], "lse")
+        within(dh, want["dh"], want["edh"], "d_hidden")
+        within(dw[1:-1], want["dw"], want["edw"], "d_weight")
+
+
 def test_strided_matrices_and_guards(torch, ctx):
     """Views with their own strides give the same bits; nothing outside the outputs is written."""
     N, V, D = 131, 777, 72
