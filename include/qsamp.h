@@ -345,7 +345,8 @@ qsamp_status qsamp_verify_greedy(qsamp_ctx* ctx, const void* logits, qsamp_dtype
  * bf16 matrices; D, every stride a multiple of 8 elements and every matrix
  * 16-byte aligned (else QSAMP_ERR_UNSUPPORTED). N = 0 is served (d_weight = 0).
  * qsamp_head_workspace: bytes either call needs for N rows (grad = 0: the
- * loss, 1: the gradients), -1 on an invalid argument. */
+ * loss, 1: the gradients), -1 on an invalid argument or a size the calls
+ * refuse. */
 typedef struct qsamp_head {
     const void* hidden;      /* DEVICE bf16 [N][hidden_stride]   */
     const void* weight;      /* DEVICE bf16 [V][weight_stride]   */

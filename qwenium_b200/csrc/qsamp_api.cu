@@ -1314,8 +1314,13 @@ qsamp_status qsamp_merge_topk(qsamp_ctx* c, int32_t n_ranks, int32_t B, int32_t 
 }
 
 // ---------------------------------------------------------------- output head
+// Coordinates of a tile's end stay in 32 bits, and so does a tile's number.
+constexpr int32_t kMaxExtent = 1 << 30;
+static bool tiles_fit(int64_t rows, int64_t cols) { return ((rows + 63) / 64) * ((cols + 63) / 64) <= INT32_MAX; }
+
 int64_t qsamp_head_workspace(const qsamp_ctx* c, int32_t N, int32_t V, int32_t D, int32_t grad) {
-    if (!c || N < 0 || V < 1 || D < 1) return -1;
+    if (!c || N < 0 || V < 1 || D < 1 || N > kMaxExtent || V > kMaxExtent || D > kMaxExtent) return -1;
+    if (!tiles_fit(N, V) || !tiles_fit(N, D) || !tiles_fit(V, D)) return -1;
     return grad ? qs_head_grad_ws(N, V, D, c->num_sms) : qs_head_loss_ws(N, V, D, c->num_sms);
 }
 
@@ -1335,17 +1340,14 @@ static qsamp_status check_matrix(qsamp_ctx* c, const char* name, const void* p, 
     return QSAMP_OK;
 }
 
-// Coordinates of a tile's end stay in 32 bits.
-constexpr int32_t kMaxExtent = 1 << 30;
 static qsamp_status check_extent(qsamp_ctx* c, const char* name, int32_t n, int32_t least) {
     if (n < least) return fail(c, QSAMP_ERR_INVALID_ARG, "%s: expected >= %d, got %d", name, least, n);
     if (n > kMaxExtent) return fail(c, QSAMP_ERR_UNSUPPORTED, "%s: expected <= %d, got %d", name, kMaxExtent, n);
     return QSAMP_OK;
 }
 
-// Tiles are numbered in 32 bits.
 static qsamp_status check_tiles(qsamp_ctx* c, int64_t rows, int64_t cols) {
-    if (((rows + 63) / 64) * ((cols + 63) / 64) > INT32_MAX)
+    if (!tiles_fit(rows, cols))
         return fail(c, QSAMP_ERR_UNSUPPORTED, "a result of %lld x %lld: more tiles than one call numbers",
                     (long long)rows, (long long)cols);
     return QSAMP_OK;

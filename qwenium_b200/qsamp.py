@@ -652,7 +652,7 @@ class Context:
 
         n = self.lib.qsamp_head_workspace(self.h, h.N, h.V, h.D, grad)
         if n < 0:
-            raise QsampError(1, f"head: expected N >= 0, V >= 1, D >= 1, got {h.N}, {h.V}, {h.D}")
+            raise QsampError(1, f"head: expected N >= 0, V >= 1, D >= 1 within one call's tiles, got {h.N}, {h.V}, {h.D}")
         return self._empty(stream, n, torch.uint8), n
 
     def head_loss(self, hidden, weight, targets, softcap: float = 0.0, stream=None):

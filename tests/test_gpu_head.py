@@ -622,3 +622,14 @@ def test_refusals(torch, ctx):
         ctx.quantize_fp8(h, block_rows=64)
     with bad:
         ctx.quantize_fp8(h.half())
+
+
+def test_workspace_of_refused_sizes(torch, ctx):
+    """Sizes no call serves, whose workspace would not fit its 64 bits either."""
+    size = lambda *a: ctx.lib.qsamp_head_workspace(ctx.h, *a)
+    top = 2**31 - 1
+    for grad in (0, 1):
+        for n, v, d in ((-1, 8, 8), (1, 0, 8), (1, 8, 0), (top, top, top), (top, 8, 8), (1, top, 8), (1, 8, top),
+                        (2**30, 8, 2**30), (8, 2**30, 2**30), (2**30, 2**30, 8)):
+            assert size(n, v, d, grad) == -1, (n, v, d, grad)
+        assert size(0, 8, 8, grad) >= 0 and size(2**22, 151936, 4096, grad) > 0
