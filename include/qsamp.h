@@ -338,8 +338,10 @@ qsamp_status qsamp_verify_greedy(qsamp_ctx* ctx, const void* logits, qsamp_dtype
  *   d_hidden = dz weight,  d_weight = dz^T hidden
  * (the last factor only with a soft-cap). dz is made again in pieces of the
  * vocabulary and rounded to bf16, the products' type (up to 64 rows: held in
- * two bf16 parts); sums and d_hidden across pieces are held in 32 bits; both gradients are rounded to bf16 once
- * at the end and overwrite their buffers. grad_loss is not read for rows
+ * two bf16 parts; more: over the mantissa of the first row's grad_loss, so
+ * that a grad_loss all rows share is not rounded); sums and d_hidden across
+ * pieces are held in 32 bits; both gradients are rounded to bf16 once at the
+ * end and overwrite their buffers. grad_loss is not read for rows
  * without a gradient.
  *
  * bf16 matrices; D, every stride a multiple of 8 elements and every matrix

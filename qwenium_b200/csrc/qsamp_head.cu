@@ -69,6 +69,7 @@ struct Params {
     float* target_logit; // [M]
     const float* lse;
     const float* grad;
+    const float* unit;   // DZ, GRAD: what dz is held over (find_unit)
     int n0;              // DZ, GRAD: first vocabulary column of the piece
     // GRAD: jobs below dh_jobs make d_hidden slabs, the rest d_weight
     int dh_jobs, d_tiles, splits, dh_k_blocks, dw_k_blocks, rows, D;
@@ -263,7 +264,7 @@ struct Epilogue<DZ> {
 
 template <>
 struct Epilogue<GRAD> {
-    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, int, float, float,
+    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, int, float, float unit,
                                 unsigned char* patch) {
         const int c0 = j.n0 + half * 128;
         if (j.second) {
@@ -276,7 +277,7 @@ struct Epilogue<GRAD> {
                     tmem_load32(tmem + c + q, v);
                     tmem_wait_load(v);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) w[(q + i) / 2] = pack_bf16(v[i], v[i + 1]);
+                    for (int i = 0; i < 32; i += 2) w[(q + i) / 2] = pack_bf16(v[i] * unit, v[i + 1] * unit);
                 }
                 store_box(&p.o, w, c0 + c, row - (int)(threadIdx.x % 32), patch);
             }
@@ -439,8 +440,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                 if (MODE == DZ && row < rows) {
                     target = p.targets[row];
                     if (target >= p.rows) target = -1;  // DZ: rows holds the vocabulary
-                    if (target >= 0) lse = p.lse[row], g = p.grad[row];
+                    if (target >= 0) lse = p.lse[row], g = __fdiv_rn(p.grad[row], *p.unit);
                 }
+                if (MODE == GRAD) g = *p.unit;
                 ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                 if (!ok) break;
                 fence_after();
@@ -1130,13 +1132,40 @@ __global__ void __launch_bounds__(1024) lse_join_kernel(const float2* part, cons
     }
 }
 
+// What dz is held over before its rounding: the mantissa, 1 to 2, of the first
+// gradient that is a normal number (1 without one). Under a mean over rows all
+// gradients are one number g, and a confident row's target has dz = -g: rounded
+// to bf16 that would be off by the same up to 2^-8 in every row, which no sum
+// averages out. Over its mantissa g is a power of two; the results are
+// multiplied by it in 32 bits. Block 0's threads look through the rows 256 at a time.
+__device__ __forceinline__ void find_unit(const int32_t* targets, const float* grad, int N, int V, float* unit) {
+    __shared__ int first;
+    if (threadIdx.x == 0) first = INT32_MAX;
+    __syncthreads();
+    for (int r0 = 0; r0 < N; r0 += 256) {
+        const int r = r0 + (int)threadIdx.x;
+        bool has = false;
+        if (r < N && targets[r] >= 0 && targets[r] < V) {
+            const uint32_t e = __float_as_uint(grad[r]) >> 23 & 255;
+            has = e > 0 && e < 255;
+        }
+        if (has) atomicMin(&first, r);
+        if (__syncthreads_or(has)) break;
+    }
+    if (threadIdx.x == 0)
+        *unit = first == INT32_MAX ? 1.0f : __uint_as_float((__float_as_uint(grad[first]) & 0x7fffffu) | 0x3f800000u);
+}
+
 // The hidden rows as d_weight's sums take them: zeros where a row has no
 // gradient, so that whatever lies there (padding, an infinity, a NaN) does not
-// meet its zero dz; parts times one below the other.
-__global__ void __launch_bounds__(256) live_rows_kernel(const uint16_t* hidden, long long stride, const int32_t* targets, int N,
-                                                        int D, int V, int parts, uint16_t* out) {
+// meet its zero dz; parts times one below the other. dz in two parts needs no
+// unit: it is 1.
+__global__ void __launch_bounds__(256) live_rows_kernel(const uint16_t* hidden, long long stride, const int32_t* targets,
+                                                        const float* grad, int N, int D, int V, int parts, uint16_t* out,
+                                                        float* unit) {
     const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8, n = (long long)N * D;
     launch_next();
+    if (blockIdx.x == 0) find_unit(targets, grad, parts == 1 ? N : 0, V, unit);
     if (i >= n) return;
     const long long row = i / D;
     const int t = targets[row];
@@ -1145,10 +1174,10 @@ __global__ void __launch_bounds__(256) live_rows_kernel(const uint16_t* hidden, 
     for (int q = 0; q < parts; ++q) *(uint4*)(out + q * n + i) = w;
 }
 
-// d_hidden = the slabs' sum (and the parts' of each) in their order, rounded
-// once; eight columns a thread.
-__global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int slices, int N, int D, uint16_t* dh,
-                                                      long long dh_stride) {
+// d_hidden = the slabs' sum (and the parts' of each) in their order, times the
+// unit, rounded once; eight columns a thread.
+__global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int slices, int N, int D, const float* unit,
+                                                      uint16_t* dh, long long dh_stride) {
     const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8, n = (long long)N * D;
     if (i >= n) return;
     wait_previous();
@@ -1157,6 +1186,9 @@ __global__ void __launch_bounds__(256) dh_join_kernel(const float* slabs, int sl
         const float4 x = *(const float4*)(slabs + s * n + i), y = *(const float4*)(slabs + s * n + i + 4);
         v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
     }
+    const float u = *unit;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] *= u;
     const uint4 w = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
     *(uint4*)(dh + i / D * dh_stride + i % D) = w;
 }
@@ -1611,7 +1643,7 @@ extern "C" long long qs_head_loss_ws(int N, int V, int, int num_sms) {
 
 extern "C" long long qs_head_grad_ws(int N, int V, int D, int num_sms) {
     const GradPlan g = grad_plan(N, V, D, num_sms);
-    return g.dz_bytes + g.slab_bytes + g.rows_bytes;
+    return g.dz_bytes + g.slab_bytes + g.rows_bytes + al(sizeof(float));
 }
 
 // The loss of at most LSE_ROWS rows.
@@ -1682,10 +1714,11 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
     uint16_t* dz = (uint16_t*)a->ws;
     float* slabs = (float*)(a->ws + g.dz_bytes);
     uint16_t* rows = (uint16_t*)(a->ws + g.dz_bytes + g.slab_bytes);
+    float* unit = (float*)(a->ws + g.dz_bytes + g.slab_bytes + g.rows_bytes);
     const int parts = grad_parts(a->N), R = a->N * parts;
     const long long n = (long long)a->N * a->D / 8;
-    live_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(a->hidden, a->hidden_stride, a->targets, a->N, a->D, a->V, parts,
-                                                                 rows);
+    live_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(a->hidden, a->hidden_stride, a->targets, a->grad_loss, a->N,
+                                                                 a->D, a->V, parts, rows, unit);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const int cols = skinny_cols(a->N, HEAD_SKINNY_ROWS);
@@ -1699,6 +1732,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.N = pw;
         p.n0 = p0;
         p.status = a->status;
+        p.unit = unit;
         if (cols) {
             SkinnyParams f = {};
             f.V = pw;
@@ -1756,8 +1790,8 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         *launches += 2;
     }
     *launches += 2;
-    return launch_after(dh_join_kernel, ceil_div(n, 256), 256, 0, st, (const float*)slabs, g.splits * parts, a->N, a->D, a->d_hidden,
-                        a->d_hidden_stride);
+    return launch_after(dh_join_kernel, ceil_div(n, 256), 256, 0, st, (const float*)slabs, g.splits * parts, a->N, a->D,
+                        (const float*)unit, a->d_hidden, a->d_hidden_stride);
 }
 
 extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {

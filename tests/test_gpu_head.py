@@ -120,6 +120,38 @@ def test_gradient_against_differences(torch, ctx):
         assert abs(diff - float(dw[v, d])) <= err + float(want["edw"][v, d])
 
 
+@pytest.mark.parametrize("N,dead", [(40, 1), (300, 1), (900, 600)])
+def test_gradients_of_a_mean(torch, ctx, N, dead):
+    """One grad_loss for all rows, in the middle between two bf16 numbers (so
+    that its own rounding would be off by 2^-8 in every row alike): the
+    targets' terms, all but the whole of the gradients here, keep their digits.
+
+    The targets' dz over grad_loss is -(1 - p), whose nearest bf16 number is
+    -1 for p <= 2^-9: off by p. The other terms are p, off by U16 p."""
+    V, D = 2000, 64
+    h, w, t, _ = H.head_inputs(N, V, D, seed=17, scale=0.01, device="cuda")
+    t[:dead] = -1  # rows without a gradient, whose grad_loss is not read
+    t[dead // 2 + 1:dead] = 5  # rows whose gradient is 0
+    g = torch.full((N,), 1.0 + 2.0**-8, device="cuda")
+    g[:dead] = float("nan")
+    g[dead // 2 + 1:dead] = 0.0
+    want = H.head_exact(h, w, t, g, 0.0)
+    _, lse = ctx.head_loss(h, w, t)
+    dh, dw = ctx.head_loss_grad(h, w, t, lse, g)
+    g = torch.where(t >= 0, g, 0.0)
+    p = torch.exp(h.double() @ w.double().t() - want["lse"].unsqueeze(1))
+    assert p.max() < 2.0**-9
+    live = (t >= 0).unsqueeze(1)
+    hot = torch.zeros_like(p).scatter_(1, t.long().clamp(min=0).unsqueeze(1), 1.0)
+    # 2^-15: the exponentials and sums of p in 32 bits, relative (p itself is below 2^-9)
+    edz = torch.where(live, g.double().unsqueeze(1) * (hot * p + (1 - hot) * p * (H.U16 + 2.0**-15) + 2.0**-9 * 2.0**-15), 0.0)
+    dz = torch.where(live, g.double().unsqueeze(1) * (p + hot), 0.0)
+    edh = (1 + H.U16) * edz @ w.double().abs() + (V + 64) * H.U32 * (dz @ w.double().abs()) + H.U16 * want["dh"].abs()
+    edw = (1 + H.U16) * edz.t() @ h.double().abs() + (N + 64) * H.U32 * (dz.t() @ h.double().abs()) + H.U16 * want["dw"].abs()
+    within(dh, want["dh"], edh, "d_hidden")
+    within(dw, want["dw"], edw, "d_weight")
+
+
 def test_rows_without_a_loss(torch, ctx):
     """Every row masked: zero losses and gradients, whatever grad_loss and lse hold."""
     h, w, t, g = H.head_inputs(70, 300, 64, seed=4, device="cuda")
