@@ -224,9 +224,6 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, const uint32_t
     if (lane == 0) tma_store(map, x, y, smem_addr(patch));
 }
 
-template <int MODE>
-struct Epilogue;
-
 // dz = g (exp(l - lse) - [target]) (1 - (l / cap)^2); 0 for rows without a
 // gradient. Without a cap (inv_cap 0) the slope is 1 for a logit of -infinity
 // too: y is 0 times the lowest finite number there.
@@ -235,75 +232,69 @@ __device__ __forceinline__ float dz_of(float l, float lse, float g, float inv_ca
     return none ? 0.0f : d * fmaf(-y, y, 1.0f) * g;
 }
 
-// Rounded to bf16, the type of the products dz goes into.
-template <>
-struct Epilogue<DZ> {
-    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, int target, float lse, float g,
-                                unsigned char* patch) {
-        const float inv = p.softcap > 0.0f ? 1.0f / p.softcap : 0.0f;
-        const int c0 = j.n0 + half * 128;
+// The thread's 128 columns of dz from its logits' products, rounded to bf16, the
+// type of the products dz goes into.
+__device__ __forceinline__ void dz_tile(const Params& p, const Job& j, float (&z)[128], int row, int half, int target, float lse,
+                                        float g, unsigned char* patch) {
+    const float inv = p.softcap > 0.0f ? 1.0f / p.softcap : 0.0f;
+    const int c0 = j.n0 + half * 128;
+#pragma unroll
+    for (int c = 0; c < 128; c += 64) {
+        if (c0 + c >= p.N) break;
+        uint32_t w[32];
+#pragma unroll
+        for (int q = 0; q < 64; q += 32) {
+            float(&v)[32] = reinterpret_cast<float(&)[32]>(z[c + q]);
+            logits_of(v, p.softcap);
+            const int at = target - (p.n0 + c0 + c + q);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+                w[(q + i) / 2] = pack_bf16(dz_of(v[i], lse, g, inv, at == i, target < 0),
+                                           dz_of(v[i + 1], lse, g, inv, at == i + 1, target < 0));
+        }
+        store_box(&p.o, w, c0 + c, row - (int)(threadIdx.x % 32), patch);
+    }
+}
+
+__device__ __forceinline__ void grad_tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, float unit,
+                                          unsigned char* patch) {
+    const int c0 = j.n0 + half * 128;
+    if (j.second) {
 #pragma unroll 1
-        for (int c = 0; c < 128 && c0 + c < p.N; c += 64) {
+        for (int c = 0; c < 128 && c0 + c < p.D; c += 64) {
             uint32_t w[32];
 #pragma unroll
             for (int q = 0; q < 64; q += 32) {
                 float v[32];
                 tmem_load32(tmem + c + q, v);
                 tmem_wait_load(v);
-                logits_of(v, p.softcap);
-                const int at = target - (p.n0 + c0 + c + q);
 #pragma unroll
-                for (int i = 0; i < 32; i += 2)
-                    w[(q + i) / 2] = pack_bf16(dz_of(v[i], lse, g, inv, at == i, target < 0),
-                                               dz_of(v[i + 1], lse, g, inv, at == i + 1, target < 0));
+                for (int i = 0; i < 32; i += 2) w[(q + i) / 2] = pack_bf16(v[i] * unit, v[i + 1] * unit);
             }
             store_box(&p.o, w, c0 + c, row - (int)(threadIdx.x % 32), patch);
         }
+        return;
     }
-};
-
-template <>
-struct Epilogue<GRAD> {
-    __device__ static void tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, int, float, float unit,
-                                unsigned char* patch) {
-        const int c0 = j.n0 + half * 128;
-        if (j.second) {
 #pragma unroll 1
-            for (int c = 0; c < 128 && c0 + c < p.D; c += 64) {
-                uint32_t w[32];
+    for (int c = 0; c < 128 && c0 + c < p.D; c += 32) {
+        float v[32];
+        tmem_load32(tmem + c, v);
+        tmem_wait_load(v);
+        if (row < p.rows) {
+            float* out = p.slabs + ((long long)j.split * p.rows + row) * p.D + c0 + c;
 #pragma unroll
-                for (int q = 0; q < 64; q += 32) {
-                    float v[32];
-                    tmem_load32(tmem + c + q, v);
-                    tmem_wait_load(v);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) w[(q + i) / 2] = pack_bf16(v[i] * unit, v[i + 1] * unit);
+            for (int i = 0; i < 32; i += 8) {
+                if (c0 + c + i >= p.D) break;
+                if (p.add) {
+                    const float4 x = *(const float4*)(out + i), y = *(const float4*)(out + i + 4);
+                    v[i] += x.x, v[i + 1] += x.y, v[i + 2] += x.z, v[i + 3] += x.w;
+                    v[i + 4] += y.x, v[i + 5] += y.y, v[i + 6] += y.z, v[i + 7] += y.w;
                 }
-                store_box(&p.o, w, c0 + c, row - (int)(threadIdx.x % 32), patch);
-            }
-            return;
-        }
-#pragma unroll 1
-        for (int c = 0; c < 128 && c0 + c < p.D; c += 32) {
-            float v[32];
-            tmem_load32(tmem + c, v);
-            tmem_wait_load(v);
-            if (row < p.rows) {
-                float* out = p.slabs + ((long long)j.split * p.rows + row) * p.D + c0 + c;
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (c0 + c + i >= p.D) break;
-                    if (p.add) {
-                        const float4 x = *(const float4*)(out + i), y = *(const float4*)(out + i + 4);
-                        v[i] += x.x, v[i + 1] += x.y, v[i + 2] += x.z, v[i + 3] += x.w;
-                        v[i + 4] += y.x, v[i + 5] += y.y, v[i + 6] += y.z, v[i + 7] += y.w;
-                    }
-                    store32(out + i, reinterpret_cast<const uint32_t(&)[8]>(v[i]));
-                }
+                store32(out + i, reinterpret_cast<const uint32_t(&)[8]>(v[i]));
             }
         }
     }
-};
+}
 
 // ---------------------------------------------------------------- the kernel
 template <int MODE>
@@ -433,22 +424,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
             const int row0 = j.m0 + (int)rank * 128 + quarter * 32, row = row0 + lane;
-            if constexpr (MODE == DZ || MODE == GRAD) {
-                const int rows = MODE == GRAD ? (j.second ? p.N : p.rows) : p.M;
-                int target = -1;
-                float lse = 0.0f, g = 0.0f;
-                if (MODE == DZ && row < rows) {
-                    target = p.targets[row];
-                    if (target >= p.rows) target = -1;  // DZ: rows holds the vocabulary
-                    if (target >= 0) lse = p.lse[row], g = __fdiv_rn(p.grad[row], *p.unit);
-                }
-                if (MODE == GRAD) g = *p.unit;
+            if constexpr (MODE == GRAD) {
+                const float unit = *p.unit;
                 ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                 if (!ok) break;
                 fence_after();
-                if (row0 < rows)
-                    Epilogue<MODE>::tile(p, j, tmem + (quarter << 21) + acc.slot * TILE + half * 128, row, half, target, lse, g,
-                                         patches + (warp - 2) * OUT_PATCH);
+                if (row0 < (j.second ? p.N : p.rows))
+                    grad_tile(p, j, tmem + (quarter << 21) + acc.slot * TILE + half * 128, row, half, unit,
+                              patches + (warp - 2) * OUT_PATCH);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
@@ -456,13 +439,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
             } else {
                 // the slices' sums added up in 128 registers: tensor memory cuts
                 // its sums rather than rounding them, which over D in the
-                // thousands would show in the loss
+                // thousands would show in the loss, and in the gradients, whose
+                // logits have to be the loss's (LOGIT_SLICE)
                 float sum[128];
 #pragma unroll
                 for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
                 const bool work = row0 < p.M;
                 const int slices = (j.k_blocks + p.slice - 1) / p.slice;
-                const int target = row < p.M ? p.targets[row] : -1;
+                int target = row < p.M ? p.targets[row] : -1;
+                float lse = 0.0f, g = 0.0f;
+                if (MODE == DZ) {
+                    if (target >= p.rows) target = -1;  // DZ: rows holds the vocabulary
+                    if (target >= 0) lse = p.lse[row], g = __fdiv_rn(p.grad[row], *p.unit);
+                }
                 for (int q = 0; q < slices; ++q, acc.step()) {
                     ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                     if (!ok) break;
@@ -481,7 +470,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                     __syncwarp();
                     if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
                 }
-                if (ok && work) softmax_sums(p, j, sum, row, half, row < p.M, target);
+                if (ok && work) {
+                    if constexpr (MODE == LSE)
+                        softmax_sums(p, j, sum, row, half, row < p.M, target);
+                    else
+                        dz_tile(p, j, sum, row, half, target, lse, g, patches + (warp - 2) * OUT_PATCH);
+                }
             }
         }
         // the last boxes leave shared memory, and arrive, before the CTA does
@@ -1563,11 +1557,17 @@ cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* weight, long lo
 
 // K blocks of 64 whose products are summed in tensor memory before fp32
 // registers take the sum. Tensor memory cuts each addition's last bits: the
-// lse comes out low by 0.5e-6 for every K block in a slice (0.9e-6, 3.8e-6,
-// 8e-6 measured at 2, 8, 16, whatever D). Shorter slices are free where the
-// weight's bytes bound the kernel; the pair's takes 2% more at 8 than at 16,
-// 13% at 4.
-constexpr int LSE_SLICE = 8, LSE_SKINNY_SLICE = 2;
+// lse of random logits comes out low by 0.5e-6 for every K block in a slice
+// (0.9e-6, 3.8e-6, 8e-6 measured at 2, 8, 16, whatever D), and a logit of 28
+// whose products all have one sign by 4e-4 with all of D 4160 in one slice. The
+// gradients take the loss's slices, so that their logits are the loss's to the
+// bit: what a row's logits are low by, its lse is too, and exp(l - lse) keeps
+// the digits that a confident row's target leaves of exp(l - lse) - 1. (Without
+// slices a target of loss 1e-5 had dz -4e-4 at D 4160, -9.6e-4 at D 8192.) Shorter
+// slices are free where the weight's bytes bound the kernel; the pair's loss
+// takes 2% more at 8 than at 16, 13% at 4; the pair's dz against one slice:
+// 509 x 1152 x 50021 256 against 238 us a step, 4096 x 2048 x 151936 7.94 against 7.82 ms.
+constexpr int LOGIT_SLICE = 8, LOGIT_SKINNY_SLICE = 2;
 // Measured on both sides (V 151936; few-row kernel against the pair's, us):
 // loss, D 2048: 1 row 102 / 149, 32 rows 110 / 123, 64 rows 118 / 124, 128
 // rows 156 / 126. 8-bit product, K 4096: 1 row 106 / 197, 64 rows 143 / 189,
@@ -1657,7 +1657,7 @@ static cudaError_t loss_round(const HeadCall* a, bool first, int* launches, cuda
         p.V = a->V;
         p.M = a->N;
         p.k_blocks = (int)ceil_div(a->D, 64);
-        p.slice = LSE_SKINNY_SLICE;
+        p.slice = LOGIT_SKINNY_SLICE;
         p.status = a->status;
         p.targets = a->targets;
         p.softcap = a->softcap;
@@ -1673,7 +1673,7 @@ static cudaError_t loss_round(const HeadCall* a, bool first, int* launches, cuda
         p.m_tiles = (int)ceil_div(a->N, TILE);
         p.n_tiles = (int)ceil_div(a->V, TILE);
         p.k_blocks = (int)ceil_div(a->D, 64);
-        p.slice = LSE_SLICE;
+        p.slice = LOGIT_SLICE;
         p.jobs = p.m_tiles * p.n_tiles;
         p.M = a->N;
         p.N = a->V;
@@ -1740,7 +1740,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             f.n0 = p0;
             f.M = a->N;
             f.k_blocks = (int)ceil_div(a->D, 64);
-            f.slice = f.k_blocks;
+            f.slice = LOGIT_SKINNY_SLICE;
             f.status = a->status;
             f.targets = a->targets;
             f.softcap = a->softcap;
@@ -1755,7 +1755,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             if (e == cudaSuccess) e = make_map(&p.o, dz, 2, a->N, g.piece, g.piece, 32);
             if (e != cudaSuccess) return e;
             p.k_blocks = (int)ceil_div(a->D, 64);
-            p.slice = INT32_MAX;
+            p.slice = LOGIT_SLICE;
             p.jobs = p.m_tiles * p.n_tiles;
             p.rows = a->V;
             p.targets = a->targets;

@@ -1,0 +1,131 @@
+"""The output-head operators where long sums and small differences show,
+against 64-bit results."""
+import pytest
+
+import head_cases as H
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch
+
+
+@pytest.fixture(scope="module")
+def ctx(torch):
+    from qwenium_b200 import qsamp
+
+    return qsamp.Context(0)
+
+
+def within(got, want, bound, what):
+    off = (got.double() - want).abs() - bound
+    assert not off.isnan().any() and off.max() <= 0, f"{what}: {int((off > 0).sum())} of {off.numel()} outside, by {off.max():.3g}"
+
+
+def confident_inputs(torch, N, V, D, top, cap):
+    """Row n has its target's logit at `top` and one runner-up that leaves it a
+    loss between 1e-6 and 1e-4; every target and runner-up is a token of its
+    own, all other logits lie near 0."""
+    g = torch.Generator().manual_seed(N + D)
+    h = torch.randn((N, D), generator=g)
+    h = H.bf16(h).double()
+    unit = h / (h * h).sum(dim=1, keepdim=True)
+    below = -torch.log(10.0 ** (-6 + 2 * torch.rand((N, 1), generator=g, dtype=torch.float64)))
+    second = top - below
+    first = torch.full_like(second, top)
+    if cap:
+        first, second = cap * torch.atanh(first / cap), cap * torch.atanh(second / cap)
+    w = torch.randn((V, D), generator=g) * (0.3 / D**0.5)
+    w[:N] = (unit * first).float()
+    w[N:2 * N] = (unit * second).float()
+    order = torch.randperm(V, generator=g)
+    w = H.bf16(w)[torch.argsort(order)]  # token i moves to place order[i]
+    t = order[:N].to(torch.int32)
+    return tuple(x.cuda() for x in (H.bf16(h.float()), w, t))
+
+
+@pytest.mark.parametrize("cap", [0.0, 40.0, 100.0])
+@pytest.mark.parametrize("N,D", [(3, 4160), (20, 8192), (40, 4096), (64, 2048), (65, 4160), (150, 8192), (300, 4096)])
+def test_gradients_of_confident_rows(torch, ctx, N, D, cap):
+    """Losses of 1e-6 to 1e-4: dz of the target is minus the loss, what is left of
+    exp(l - lse) - 1. The gradients make the loss's logits again, bit for bit, so
+    an error common to a row's logits cancels, and what remains is:
+
+      lse's rounding, U32 lse; the sum's (one rounding where the runner-up is
+      added, its neighbours do not move a sum of 1, and the joins of few parts) and
+      the exponentials beside 1: 24 U32 together;
+      the runner-up's distance, off by at most both logits' errors ez (D + 8 products
+      and sums; 32 U32 of the cap), times its p."""
+    top = 28.0
+    V = 2 * N + 300
+    h, w, t = confident_inputs(torch, N, V, D, top, cap)
+    g = torch.rand((N,), generator=torch.Generator().manual_seed(1)).add(0.5).cuda()
+    hd, wd = h.double(), w.double()
+    z = hd @ wd.t()
+    ez = (D + 8) * H.U32 * (hd.abs() @ wd.abs().t()).amax(dim=1)
+    slope = torch.ones_like(z)
+    if cap:
+        y = torch.tanh(z / cap)
+        z, slope = cap * y, 1 - y * y
+        ez = ez + 32 * H.U32 * cap
+    at = t.long()[:, None]
+    lse = torch.logsumexp(z, dim=1)
+    p = torch.exp(z - lse[:, None])
+    rest = p.scatter(1, at, 0.0).sum(dim=1)
+    assert (rest > 5e-7).all() and (rest < 2e-4).all()
+    dz = p.scatter(1, at, -rest[:, None]) * slope * g.double()[:, None]
+    loss, lse32 = ctx.head_loss(h, w, t, softcap=cap)
+    dh, dw = ctx.head_loss_grad(h, w, t, lse32, g, softcap=cap)
+    e = (lse + 24) * H.U32
+    hot = torch.zeros_like(p).scatter_(1, at, 1.0)
+    # the target's dz, and the runner-up's (p times twice its errors); the slope is off by 2 ez / cap + 8 U32
+    edz = hot * (e + 2 * ez * rest)[:, None] + (1 - hot) * p * (2 * ez + e)[:, None]
+    edz = edz * slope * g.double()[:, None] + dz.abs() * (H.U16**2 if N <= 64 else H.U16)
+    if cap:
+        edz = edz + dz.abs() / slope * (2 * ez / cap + 8 * H.U32)[:, None]
+    edz = edz + 2.0**-126
+    loose = 1 + 2 * H.U16
+    # d_weight of a target: its own row, and p of the others
+    want = dz.t() @ hd
+    bound = edz.t() @ hd.abs() * loose + (N + 64) * H.U32 * (dz.abs().t() @ hd.abs()) + H.U16 * want.abs()
+    rows = t.long()
+    within(dw[rows], want[rows], bound[rows], "d_weight of the targets")
+    within(dw, want, bound, "d_weight")
+    want = dz @ wd
+    bound = edz @ wd.abs() * loose + (V + 64) * H.U32 * (dz.abs() @ wd.abs()) + H.U16 * want.abs()
+    within(dh, want, bound, "d_hidden")
+    # and the loss itself: lse's rounding, the target's logit is the largest
+    within(loss, lse - z.gather(1, at)[:, 0], e + 2 * ez * rest, "loss")
+
+
+@pytest.mark.parametrize("N,D", [(50, 64), (150, 64), (50, 4096), (150, 4096)])
+def test_gradients_of_large_logits(torch, ctx, N, D):
+    """Logits of a few thousand, rows whose largest is 60 above the next: lse is
+    that logit to the bit (logf(1) is 0), p is 1 there and 0 elsewhere, so dz is g
+    at the largest, -g at the target, and at most 8 U32 g where they meet."""
+    V = 2000
+    h, w, t, g = H.head_inputs(N, V, D, seed=6, scale=2000.0, ignored=0.0, device="cuda")
+    hd, wd = h.double(), w.double()
+    top2, arg = (hd @ wd.t()).topk(2, dim=1)
+    clear = top2[:, 0] - top2[:, 1] > 60
+    assert clear.sum() > N // 2
+    t = torch.where(torch.arange(N, device="cuda") % 3 == 0, arg[:, 0].to(torch.int32), t)  # some are their targets
+    t = torch.where(clear, t, -1)
+    _, lse = ctx.head_loss(h, w, t)
+    dh, dw = ctx.head_loss_grad(h, w, t, lse, g)
+    gr = torch.where(t >= 0, g, 0.0).double()[:, None]
+    hot = torch.zeros((N, V), dtype=torch.float64, device="cuda").scatter_(1, t.long().clamp(min=0)[:, None], 1.0)
+    p = torch.zeros_like(hot).scatter_(1, arg[:, :1], 1.0)
+    dz = (p - hot) * gr
+    edz = dz.abs() * (H.U16**2 if N <= 64 else H.U16) + 8 * H.U32 * (p + hot) * gr.abs() + 2.0**-80
+    loose = 1 + 2 * H.U16
+    want = dz @ wd
+    within(dh, want, edz @ wd.abs() * loose + (V + 64) * H.U32 * (dz.abs() @ wd.abs()) + H.U16 * want.abs(), "d_hidden")
+    want = dz.t() @ hd
+    within(dw, want, edz.t() @ hd.abs() * loose + (N + 64) * H.U32 * (dz.abs().t() @ hd.abs()) + H.U16 * want.abs(), "d_weight")
