@@ -340,11 +340,12 @@ qsamp_status qsamp_verify_greedy(qsamp_ctx* ctx, const void* logits, qsamp_dtype
  * of the vocabulary, to the bit those of qsamp_head_loss for the same N, so
  * that a confident row's exp(l - lse) - 1 keeps its digits down to lse's own
  * rounding; an lse from elsewhere, or of the rows in calls of other N, is
- * served, and off from these logits by their sums' rounding. dz is rounded to bf16, the products' type (up to 64 rows: held in
- * two bf16 parts; more: over the mantissa of the first row's grad_loss, so
- * that a grad_loss all rows share is not rounded); sums and d_hidden across
- * pieces are held in 32 bits; both gradients are rounded to bf16 once at the
- * end and overwrite their buffers. grad_loss is not read for rows
+ * served, and off from these logits by their sums' rounding. dz is rounded to
+ * bf16, the products' type (up to 64 rows: held in two bf16 parts; more: over
+ * the mantissa of the first row's grad_loss, so that a grad_loss all rows
+ * share is not rounded); sums and d_hidden across pieces are held in 32 bits;
+ * both gradients are rounded to bf16 once at the end and overwrite their
+ * buffers. grad_loss is not read for rows
  * without a gradient.
  *
  * bf16 matrices; D, every stride a multiple of 8 elements and every matrix

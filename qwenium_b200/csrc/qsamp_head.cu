@@ -1579,9 +1579,7 @@ constexpr int FP8_SKINNY_ROWS = 128;
 constexpr int LSE_ROWS = 16384;
 
 // Partial sums a row's logits come in.
-long long lse_parts(int N, int V, int num_sms) {
-    return skinny_cols(N, HEAD_SKINNY_ROWS) ? 4ll * num_sms : 2 * ceil_div(V, TILE);
-}
+long long lse_parts(bool few, int V, int num_sms) { return few ? 4ll * num_sms : 2 * ceil_div(V, TILE); }
 
 // How the gradients are cut: the vocabulary into equal pieces whose dz takes
 // at most DZ_BYTES, and each piece's d_hidden sums into splits along the
@@ -1638,7 +1636,7 @@ using namespace qs;
 
 extern "C" long long qs_head_loss_ws(int N, int V, int, int num_sms) {
     const long long rows = N < LSE_ROWS ? N : LSE_ROWS;
-    return al(8 * rows * lse_parts(N, V, num_sms)) + al(4 * rows);
+    return al(8 * rows * lse_parts(skinny_cols(N, HEAD_SKINNY_ROWS) != 0, V, num_sms)) + al(4 * rows);
 }
 
 extern "C" long long qs_head_grad_ws(int N, int V, int D, int num_sms) {
@@ -1646,13 +1644,15 @@ extern "C" long long qs_head_grad_ws(int N, int V, int D, int num_sms) {
     return g.dz_bytes + g.slab_bytes + g.rows_bytes + al(sizeof(float));
 }
 
-// The loss of at most LSE_ROWS rows.
-static cudaError_t loss_round(const HeadCall* a, bool first, int* launches, cudaStream_t st) {
+// The loss of at most LSE_ROWS rows. All rounds of a call take the same kernel
+// (cols: the few-row one's): a row's bits, which the gradients make again, do
+// not depend on its round, and the workspace has one layout.
+static cudaError_t loss_round(const HeadCall* a, int cols, bool first, int* launches, cudaStream_t st) {
     float2* part = (float2*)a->ws;
-    float* target_logit = (float*)(a->ws + al(8ll * a->N * lse_parts(a->N, a->V, a->num_sms)));
+    float* target_logit = (float*)(a->ws + al(8ll * a->N * lse_parts(cols != 0, a->V, a->num_sms)));
     int parts;
     cudaError_t e;
-    if (const int cols = skinny_cols(a->N, HEAD_SKINNY_ROWS)) {
+    if (cols) {
         SkinnyParams p = {};
         p.V = a->V;
         p.M = a->N;
@@ -1700,7 +1700,7 @@ extern "C" cudaError_t qs_head_loss(const HeadCall* a, int* launches, cudaStream
         part.loss += r;
         part.lse_out += r;
         part.N = (int)(a->N - r < LSE_ROWS ? a->N - r : LSE_ROWS);
-        const cudaError_t e = loss_round(&part, r == 0, launches, st);
+        const cudaError_t e = loss_round(&part, skinny_cols(a->N, HEAD_SKINNY_ROWS), r == 0, launches, st);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;

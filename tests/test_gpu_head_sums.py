@@ -129,3 +129,14 @@ def test_gradients_of_large_logits(torch, ctx, N, D):
     within(dh, want, edz @ wd.abs() * loose + (V + 64) * H.U32 * (dz.abs() @ wd.abs()) + H.U16 * want.abs(), "d_hidden")
     want = dz.t() @ hd
     within(dw, want, edz.t() @ hd.abs() * loose + (N + 64) * H.U32 * (dz.abs().t() @ hd.abs()) + H.U16 * want.abs(), "d_weight")
+
+
+@pytest.mark.parametrize("more", [1, 40, 64])
+def test_a_last_round_of_few_rows(torch, ctx, more):
+    """Rows past a round of partial sums: a row's bits are those it has in the
+    first round, however few rows the last one holds."""
+    D, V = 2048, 200
+    h, w, t, _ = H.head_inputs(16384, V, D, seed=18, device="cuda")
+    h, t = torch.cat([h, h[:more]]), torch.cat([t, t[:more]])
+    loss, lse = ctx.head_loss(h, w, t)
+    assert torch.equal(lse[16384:], lse[:more]) and torch.equal(loss[16384:], loss[:more])
