@@ -256,22 +256,45 @@ __device__ __forceinline__ void dz_tile(const Params& p, const Job& j, float (&z
     }
 }
 
+// 64 columns of d_weight, from column c.
+__device__ __forceinline__ void store_dw(const Params& p, float (&v)[64], int c, int row, float unit, unsigned char* patch) {
+    uint32_t w[32];
+#pragma unroll
+    for (int i = 0; i < 64; i += 2) w[i / 2] = pack_bf16(v[i] * unit, v[i + 1] * unit);
+    store_box(&p.o, w, c, row - (int)(threadIdx.x % 32), patch);
+}
+
+// 32 columns of a d_hidden slab, from column c.
+__device__ __forceinline__ void store_dh(const Params& p, const Job& j, float (&v)[32], int c, int row) {
+    if (row >= p.rows) return;
+    float* out = p.slabs + ((long long)j.split * p.rows + row) * p.D + c;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        if (c + i >= p.D) break;
+        if (p.add) {
+            const float4 x = *(const float4*)(out + i), y = *(const float4*)(out + i + 4);
+            v[i] += x.x, v[i + 1] += x.y, v[i + 2] += x.z, v[i + 3] += x.w;
+            v[i + 4] += y.x, v[i + 5] += y.y, v[i + 6] += y.z, v[i + 7] += y.w;
+        }
+        store32(out + i, reinterpret_cast<const uint32_t(&)[8]>(v[i]));
+    }
+}
+
+// The thread's 128 columns of either gradient, straight from tensor memory.
 __device__ __forceinline__ void grad_tile(const Params& p, const Job& j, uint32_t tmem, int row, int half, float unit,
                                           unsigned char* patch) {
     const int c0 = j.n0 + half * 128;
     if (j.second) {
 #pragma unroll 1
         for (int c = 0; c < 128 && c0 + c < p.D; c += 64) {
-            uint32_t w[32];
+            float v[64];
 #pragma unroll
             for (int q = 0; q < 64; q += 32) {
-                float v[32];
-                tmem_load32(tmem + c + q, v);
-                tmem_wait_load(v);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) w[(q + i) / 2] = pack_bf16(v[i] * unit, v[i + 1] * unit);
+                float(&part)[32] = reinterpret_cast<float(&)[32]>(v[q]);
+                tmem_load32(tmem + c + q, part);
+                tmem_wait_load(part);
             }
-            store_box(&p.o, w, c0 + c, row - (int)(threadIdx.x % 32), patch);
+            store_dw(p, v, c0 + c, row, unit, patch);
         }
         return;
     }
@@ -280,24 +303,27 @@ __device__ __forceinline__ void grad_tile(const Params& p, const Job& j, uint32_
         float v[32];
         tmem_load32(tmem + c, v);
         tmem_wait_load(v);
-        if (row < p.rows) {
-            float* out = p.slabs + ((long long)j.split * p.rows + row) * p.D + c0 + c;
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-                if (c0 + c + i >= p.D) break;
-                if (p.add) {
-                    const float4 x = *(const float4*)(out + i), y = *(const float4*)(out + i + 4);
-                    v[i] += x.x, v[i + 1] += x.y, v[i + 2] += x.z, v[i + 3] += x.w;
-                    v[i + 4] += y.x, v[i + 5] += y.y, v[i + 6] += y.z, v[i + 7] += y.w;
-                }
-                store32(out + i, reinterpret_cast<const uint32_t(&)[8]>(v[i]));
-            }
-        }
+        store_dh(p, j, v, c0 + c, row);
     }
+}
+// The same from the sum of several slices.
+__device__ __forceinline__ void grad_tile(const Params& p, const Job& j, float (&z)[128], int row, int half, float unit,
+                                          unsigned char* patch) {
+    const int c0 = j.n0 + half * 128;
+    if (j.second) {
+#pragma unroll
+        for (int c = 0; c < 128; c += 64)
+            if (c0 + c < p.D) store_dw(p, reinterpret_cast<float(&)[64]>(z[c]), c0 + c, row, unit, patch);
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < 128; c += 32)
+        if (c0 + c < p.D) store_dh(p, j, reinterpret_cast<float(&)[32]>(z[c]), c0 + c, row);
 }
 
 // ---------------------------------------------------------------- the kernel
-template <int MODE>
+// SLICED: an accumulator may hold part of a tile's sums (p.slice K blocks).
+template <int MODE, bool SLICED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_kernel(const __grid_constant__ Params p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -424,58 +450,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             const Job j = job_of<MODE>(p, job);
             const int row0 = j.m0 + (int)rank * 128 + quarter * 32, row = row0 + lane;
-            if constexpr (MODE == GRAD) {
+            const int rows = MODE != GRAD ? p.M : j.second ? p.N : p.rows;
+            const bool work = row0 < rows;
+            unsigned char* patch = patches + (warp - 2) * OUT_PATCH;
+            if constexpr (!SLICED) {
                 const float unit = *p.unit;
                 ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
                 if (!ok) break;
                 fence_after();
-                if (row0 < (j.second ? p.N : p.rows))
-                    grad_tile(p, j, tmem + (quarter << 21) + acc.slot * TILE + half * 128, row, half, unit,
-                              patches + (warp - 2) * OUT_PATCH);
+                if (work) grad_tile(p, j, tmem + (quarter << 21) + acc.slot * TILE + half * 128, row, half, unit, patch);
                 fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
                 acc.step();
-            } else {
-                // the slices' sums added up in 128 registers: tensor memory cuts
-                // its sums rather than rounding them, which over D in the
-                // thousands would show in the loss, and in the gradients, whose
-                // logits have to be the loss's (LOGIT_SLICE)
-                float sum[128];
+                continue;
+            }
+            int target = -1;
+            float lse = 0.0f, g = 0.0f;
+            if (MODE == GRAD) g = *p.unit;
+            if (MODE != GRAD && row < rows) target = p.targets[row];
+            if (MODE == DZ) {
+                if (target >= p.rows) target = -1;  // DZ: rows holds the vocabulary
+                if (target >= 0) lse = p.lse[row], g = __fdiv_rn(p.grad[row], *p.unit);
+            }
+            const int slices = (j.k_blocks - 1) / p.slice + 1;
+            // the slices' sums added up in 128 registers: tensor memory cuts its
+            // sums rather than rounding them (LOGIT_SLICE, GRAD_SLICE)
+            float sum[128];
 #pragma unroll
-                for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
-                const bool work = row0 < p.M;
-                const int slices = (j.k_blocks + p.slice - 1) / p.slice;
-                int target = row < p.M ? p.targets[row] : -1;
-                float lse = 0.0f, g = 0.0f;
-                if (MODE == DZ) {
-                    if (target >= p.rows) target = -1;  // DZ: rows holds the vocabulary
-                    if (target >= 0) lse = p.lse[row], g = __fdiv_rn(p.grad[row], *p.unit);
-                }
-                for (int q = 0; q < slices; ++q, acc.step()) {
-                    ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
-                    if (!ok) break;
-                    fence_after();
-                    if (work) {
+            for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
+            for (int q = 0; q < slices; ++q, acc.step()) {
+                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
+                if (!ok) break;
+                fence_after();
+                if (work) {
 #pragma unroll
-                        for (int c = 0; c < 128; c += 32) {
-                            float v[32];
-                            tmem_load32(tmem + (quarter << 21) + acc.slot * TILE + half * 128 + c, v);
-                            tmem_wait_load(v);
+                    for (int c = 0; c < 128; c += 32) {
+                        float v[32];
+                        tmem_load32(tmem + (quarter << 21) + acc.slot * TILE + half * 128 + c, v);
+                        tmem_wait_load(v);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sum[c + i] += v[i];
-                        }
+                        for (int i = 0; i < 32; ++i) sum[c + i] += v[i];
                     }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
                 }
-                if (ok && work) {
-                    if constexpr (MODE == LSE)
-                        softmax_sums(p, j, sum, row, half, row < p.M, target);
-                    else
-                        dz_tile(p, j, sum, row, half, target, lse, g, patches + (warp - 2) * OUT_PATCH);
-                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive_cluster(lead_empty0 + 8 * acc.slot);
+            }
+            if (!ok) break;
+            if (work) {
+                if constexpr (MODE == LSE)
+                    softmax_sums(p, j, sum, row, half, row < rows, target);
+                else if constexpr (MODE == DZ)
+                    dz_tile(p, j, sum, row, half, target, lse, g, patch);
+                else
+                    grad_tile(p, j, sum, row, half, g, patch);
             }
         }
         // the last boxes leave shared memory, and arrive, before the CTA does
@@ -1486,10 +1515,10 @@ cudaError_t allow_smem(K* kernel, int bytes, int bit, uint32_t* ready) {
     return e;
 }
 // Bits: the pair kernel's modes 0 to 2, the wide kernel 3, the few-row kernel's
-// modes times column counts from 4.
-constexpr int WIDE_BIT = 3;
+// modes times column counts from 4, the pair kernel without slices 31.
+constexpr int WIDE_BIT = 3, WHOLE_BIT = 31;
 constexpr int skinny_bit(int mode, int cols) { return 4 + mode * 4 + (cols == 16 ? 0 : cols == 32 ? 1 : cols == 64 ? 2 : 3); }
-static_assert(skinny_bit(FP8, 128) < 32, "bits of a word");
+static_assert(skinny_bit(FP8, 128) < WHOLE_BIT, "bits of a word");
 
 // A launch that may begin before the call's previous kernel has ended (the
 // kernel calls wait_previous).
@@ -1508,14 +1537,14 @@ cudaError_t launch_after(void (*kernel)(A...), long long blocks, int threads, in
     return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
-template <int MODE>
+template <int MODE, bool SLICED = true>
 cudaError_t launch(const Params& p, const HeadCall* a, bool first, cudaStream_t st) {
     constexpr int smem = smem_bytes(MODE);
-    const cudaError_t e = allow_smem(head_kernel<MODE>, smem, MODE, a->ready);
+    const cudaError_t e = allow_smem(head_kernel<MODE, SLICED>, smem, SLICED ? MODE : WHOLE_BIT, a->ready);
     if (e != cudaSuccess) return e;
     const int pairs = a->num_sms / 2 < p.jobs ? a->num_sms / 2 : p.jobs;
-    if (!first) return launch_after(head_kernel<MODE>, 2 * pairs, THREADS, smem, st, p);
-    head_kernel<MODE><<<2 * pairs, THREADS, smem, st>>>(p);
+    if (!first) return launch_after(head_kernel<MODE, SLICED>, 2 * pairs, THREADS, smem, st, p);
+    head_kernel<MODE, SLICED><<<2 * pairs, THREADS, smem, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -1568,6 +1597,13 @@ cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* weight, long lo
 // takes 2% more at 8 than at 16, 13% at 4; the pair's dz against one slice:
 // 509 x 1152 x 50021 256 against 238 us a step, 4096 x 2048 x 151936 7.94 against 7.82 ms.
 constexpr int LOGIT_SLICE = 8, LOGIT_SKINNY_SLICE = 2;
+// The gradients' sums, over the rows (d_weight) and over a split of the
+// vocabulary (d_hidden), stay in tensor memory for at most 32768 products. A sum
+// of one sign comes out low by 1e-7 of itself per 16 products (1.2e-2 after 2^21
+// rows in one slice): 2e-4 here, where the rounding to bf16 is up to 4e-3. Calls
+// of no longer sums run the kernel without slices, which at the same sizes takes
+// 2% (4096 x 2048 x 151936) to 10% (4 x 2048 x 151936) less.
+constexpr int GRAD_SLICE = 512;
 // Measured on both sides (V 151936; few-row kernel against the pair's, us):
 // loss, D 2048: 1 row 102 / 149, 32 rows 110 / 123, 64 rows 118 / 124, 128
 // rows 156 / 126. 8-bit product, K 4096: 1 row 106 / 197, 64 rows 143 / 189,
@@ -1588,7 +1624,7 @@ long long lse_parts(bool few, int V, int num_sms) { return few ? 4ll * num_sms :
 // mod pairs, d_hidden's first: r pairs have one d_hidden job more, and the
 // d_weight jobs left over go to the pairs from r on. Every split's slab is read
 // and written per piece, so there are at most four jobs a pair of them.
-constexpr long long DZ_BYTES = 256ll << 20;
+constexpr long long DZ_BYTES = 256ll << 20;  // but at least TILE columns: more above 524288 rows
 constexpr int MAX_SPLITS = 32;
 struct GradPlan {
     int piece, pieces, splits;
@@ -1773,7 +1809,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         if (e == cudaSuccess)
             e = make_map(&p.o, a->d_weight + (long long)p0 * a->d_weight_stride, 2, pw, a->D, a->d_weight_stride, 32);
         if (e != cudaSuccess) return e;
-        p.slice = INT32_MAX;
+        p.slice = GRAD_SLICE;
         p.d_tiles = (int)ceil_div(a->D, TILE);
         p.dh_k_blocks = (int)ceil_div(pw, 64);
         // every split has a K block; a short last piece adds to the first slabs
@@ -1785,7 +1821,8 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.D = a->D;
         p.slabs = slabs;
         p.add = q > 0;
-        e = launch<GRAD>(p, a, false, st);
+        const bool whole = p.dw_k_blocks <= GRAD_SLICE && ceil_div(p.dh_k_blocks, p.splits) <= GRAD_SLICE;
+        e = whole ? launch<GRAD, false>(p, a, false, st) : launch<GRAD>(p, a, false, st);
         if (e != cudaSuccess) return e;
         *launches += 2;
     }

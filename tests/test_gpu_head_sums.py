@@ -140,3 +140,53 @@ def test_a_last_round_of_few_rows(torch, ctx, more):
     h, t = torch.cat([h, h[:more]]), torch.cat([t, t[:more]])
     loss, lse = ctx.head_loss(h, w, t)
     assert torch.equal(lse[16384:], lse[:more]) and torch.equal(loss[16384:], loss[:more])
+
+
+def test_a_long_sum_of_one_sign(torch, ctx):
+    """d_weight over 2^22 rows whose terms have one sign: logits 0, so dz is -7/8
+    and 1/8 to the bit. In tensor memory an addition cuts 16 products and the sum
+    so far, each by at most 2^-23 of that sum: over a slice of 2048 additions, the
+    sum half its last on average, 17 * 2^-13 of it; the slices' sum adds 128 U32;
+    one rounding to bf16. (2^21 rows in one slice came out low by 1.2e-2.)"""
+    N, V, D = 2**22, 8, 64
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    h = (torch.rand((N, D), generator=gen, device="cuda") * 0.5 + 0.5).to(torch.bfloat16)
+    w = torch.zeros((V, D), dtype=torch.bfloat16, device="cuda")
+    t = torch.zeros((N,), dtype=torch.int32, device="cuda")
+    _, lse = ctx.head_loss(h, w, t)
+    _, dw = ctx.head_loss_grad(h, w, t, lse, torch.ones((N,), device="cuda"))
+    total = h.double().sum(dim=0)
+    # exp(-lse) is within 8 U32 of 1/8, and so rounds to it
+    want = torch.cat([-0.875 * total[None], 0.125 * total[None].expand(V - 1, D)])
+    bound = (H.U16 + (17 * 2.0**-13 + 128 * H.U32) * (1 + H.U16)) * want.abs()
+    within(dw, want, bound, "d_weight")
+
+
+def test_long_sums_over_the_vocabulary(torch, ctx):
+    """d_hidden in two pieces of the vocabulary whose sums are several slices each
+    (many tiles of d_hidden leave no room for splits), d_weight beside it in one;
+    the last piece's rows, one of them a target, among d_weight's."""
+    if torch.cuda.mem_get_info()[0] < 40 * 2**30:
+        pytest.skip("needs 40 GB")
+    N, V, D = 1100, 200000, 8200
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    w = torch.empty((V, D), dtype=torch.bfloat16, device="cuda")
+    for r in range(0, V, 20000):
+        w[r:r + 20000] = torch.randn((20000, D), generator=gen, device="cuda") * (2.0 / D**0.5)
+    h = torch.randn((N, D), generator=gen, device="cuda").to(torch.bfloat16)
+    t = torch.randint(0, V, (N,), generator=gen, device="cuda").to(torch.int32)
+    t[0], t[5] = V - 1, -1
+    g = torch.rand((N,), generator=gen, device="cuda") + 0.5
+    z = torch.cat([h.double() @ w[r:r + 20000].double().t() for r in range(0, V, 20000)], dim=1)
+    lse64 = torch.logsumexp(z, dim=1)
+    _, lse = ctx.head_loss(h, w, t)
+    dh, dw = ctx.head_loss_grad(h, w, t, lse, g)
+    dz = torch.exp(z - lse64[:, None])
+    dz.scatter_add_(1, t.long().clamp(min=0)[:, None], torch.full((N, 1), -1.0, dtype=torch.float64, device="cuda"))
+    dz *= torch.where(t >= 0, g, 0.0).double()[:, None]
+    want = sum(dz[:, r:r + 20000] @ w[r:r + 20000].double() for r in range(0, V, 20000))
+    # two independent roundings of half a bf16 step each stay below twice one of them
+    assert (dh.double() - want).norm() <= 2 * H.U16 * want.norm() and (dh[5] == 0).all()
+    for a in (0, 100000 - 1000, V - 2000):
+        want = dz[:, a:a + 2000].t() @ h.double()
+        assert (dw[a:a + 2000].double() - want).norm() <= 2 * H.U16 * want.norm()
