@@ -190,3 +190,33 @@ def test_long_sums_over_the_vocabulary(torch, ctx):
     for a in (0, 100000 - 1000, V - 2000):
         want = dz[:, a:a + 2000].t() @ h.double()
         assert (dw[a:a + 2000].double() - want).norm() <= 2 * H.U16 * want.norm()
+
+
+def rounded_e4m3(torch, y):
+    """Doubles to the nearest e4m3 value, ties to even, saturated."""
+    y = y.clamp(-448.0, 448.0)
+    step = torch.ldexp(torch.ones_like(y), torch.frexp(y.abs())[1].sub(1).clamp(min=-6).sub(3))
+    return torch.round(y / step) * step
+
+
+@pytest.mark.parametrize("rows,M", [(1, 65535 * 32 + 33), (128, 65535 * 128 + 129)])
+def test_quantiser_rows_past_the_grid(torch, ctx, rows, M):
+    """More groups of rows (32, or a square block) than a grid's second dimension
+    holds: its blocks take a second group. Every group has its own scale."""
+    K = 16
+    if torch.cuda.mem_get_info()[0] < 20 * 2**30:
+        pytest.skip("needs 20 GB")
+    r = torch.arange(M, device="cuda")
+    x = torch.rand((M, K), generator=torch.Generator(device="cuda").manual_seed(20), device="cuda") - 0.5
+    x *= torch.ldexp(1 + (r // rows % 127).float() / 128, (r // rows % 41 - 20).to(torch.int32))[:, None]
+    x = x.to(torch.bfloat16)
+    q, s = ctx.quantize_fp8(x, block_rows=rows)
+    blocks = -(-M // rows)
+    top = torch.zeros((blocks * rows,), dtype=torch.float64, device="cuda")
+    top[:M] = x.abs().amax(dim=1).double()
+    top = top.view(blocks, rows).amax(dim=1, keepdim=True)
+    assert torch.equal(s, (top / torch.full_like(top, 448.0)).float())
+    for a in range(0, M, 2**20):
+        b = min(a + 2**20, M)
+        want = rounded_e4m3(torch, x[a:b].double() / s[r[a:b] // rows].double())
+        assert torch.equal(q[a:b].double(), want), f"rows {a} to {b}"
