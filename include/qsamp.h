@@ -318,9 +318,14 @@ qsamp_status qsamp_verify_greedy(qsamp_ctx* ctx, const void* logits, qsamp_dtype
  * the same call every time. Buffers are DEVICE memory, borrowed for the call;
  * outputs must not overlap inputs or the workspace. The workspace belongs to
  * the caller, 256-byte aligned: two calls that may overlap on the GPU (two
- * streams, two captured graphs) need one each. A bounded wait that ran out
- * in one of these kernels is reported by qsamp_poll_status (QSAMP_ERR_DEVICE,
- * once); the outputs of the calls since the last report are then invalid.
+ * streams, two captured graphs) need one each.
+ *
+ * The parts of these kernels wait for one another with a bound, two seconds
+ * or what qsamp_set_head_wait says (qsamp_set_limits' bounds are the
+ * selection's). A wait that ran out ends the kernel and is reported by
+ * qsamp_poll_status (QSAMP_ERR_DEVICE, once) after the stream was
+ * synchronised; the outputs of the calls since the last report are then
+ * invalid.
  *
  * Cross entropy of N hidden rows under a head weight, without the [N][V]
  * logits in memory:
@@ -361,6 +366,10 @@ typedef struct qsamp_head {
     int64_t hidden_stride, weight_stride; /* elements, >= D      */
     float softcap;           /* 0: off; 2^-60 to 2^60            */
 } qsamp_head;
+/* The bound of the waits in the output-head kernels launched from now on, in
+ * nanoseconds (a captured graph keeps its own); 0 (tests): the matrix
+ * instructions do not wait for the first operands, and all else runs out. */
+qsamp_status qsamp_set_head_wait(qsamp_ctx* ctx, int64_t ns);
 int64_t qsamp_head_workspace(const qsamp_ctx* ctx, int32_t N, int32_t V, int32_t D, int32_t grad);
 qsamp_status qsamp_head_loss(qsamp_ctx* ctx, const qsamp_head* head, float* out_loss, float* out_lse, void* workspace,
                              int64_t workspace_bytes, void* stream);

@@ -101,14 +101,30 @@ __device__ __forceinline__ unsigned long long now_ns() {
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Longest wait of a role for another; a kernel's own copies and matrix
-// instructions finish in microseconds.
-constexpr unsigned long long WAIT_NS = 2000000000ull;
+// How long a role waits for another: a kernel's own copies and matrix
+// instructions finish in microseconds. When a wait runs out, *gave_up (shared
+// memory of the CTA) and *status (mapped host memory) are set.
+struct Patience {
+    volatile int* gave_up;
+    int* status;
+    unsigned long long ns;
+    __device__ __forceinline__ void run_out() const {
+        *gave_up = 1;
+        *(volatile int*)status = 1;
+    }
+};
 
 // Waits for the barrier's phase. False when the wait ran out, or another role
-// of this CTA gave up: *gave_up (shared memory) and *status (mapped host
-// memory) are set, and the caller leaves its loop.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
+// of this CTA gave up: the caller leaves its loop. ISSUER (the warp of the matrix
+// instructions, on whose progress the others' waits depend): without any time to
+// wait, a phase that is not over when it is asked for has run out.
+template <bool ISSUER>
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const Patience& w) {
+    if (ISSUER && w.ns == 0) {
+        if (bar_test(bar, parity)) return true;
+        w.run_out();
+        return false;
+    }
     // the clock is slow to read: the short waits of a running pipeline end before it is
     for (int spin = 0; spin < 256; ++spin)
         if (bar_try(bar, parity)) return true;
@@ -116,10 +132,9 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     for (uint32_t spin = 1;; ++spin) {
         if (bar_try(bar, parity)) return true;
         if ((spin & 63) == 0) {
-            if (*gave_up) return false;
-            if (now_ns() - t0 > WAIT_NS) {
-                *gave_up = 1;
-                *(volatile int*)status = 1;
+            if (*w.gave_up) return false;
+            if (now_ns() - t0 > w.ns) {
+                w.run_out();
                 return false;
             }
         }
@@ -127,8 +142,21 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 }
 
 // The same for a converged warp: the answer is the warp's.
-__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
-    return __all_sync(0xffffffffu, bar_wait(bar, parity, gave_up, status));
+template <bool ISSUER = false>
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, const Patience& w) {
+    return __all_sync(0xffffffffu, bar_wait<ISSUER>(bar, parity, w));
+}
+
+// Before a CTA leaves: after a role gave up, whatever the CTA had in flight
+// (copies, matrix instructions: microseconds) lands while it is here. The clock
+// decides, for a sleep may return at once; the count is its own bound.
+__device__ __forceinline__ void let_land(const Patience& w) {
+    __syncwarp();
+    if (*w.gave_up) {
+        const unsigned long long t0 = now_ns();
+        for (int i = 0; i < 100000 && now_ns() - t0 < 20000000ull; ++i) __nanosleep(1000);
+    }
+    __syncwarp();
 }
 
 // Position in a ring of N barriers: the slot and the parity of its phase,

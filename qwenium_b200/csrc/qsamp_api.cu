@@ -116,6 +116,7 @@ struct qsamp_ctx {
     // out (they have no per-call status to clear or copy); read and cleared by
     // qsamp_poll_status
     int* head_status = nullptr;
+    unsigned long long head_wait_ns = 2000000000ull;  // how long their waits may take (qsamp_set_head_wait)
     uint32_t head_ready = 0;  // output-head kernels whose attributes are set on this device
     // device-side bounds (qsamp_set_limits)
     int max_rounds = kMaxRounds;
@@ -1324,6 +1325,14 @@ int64_t qsamp_head_workspace(const qsamp_ctx* c, int32_t N, int32_t V, int32_t D
     return grad ? qs_head_grad_ws(N, V, D, c->num_sms) : qs_head_loss_ws(N, V, D, c->num_sms);
 }
 
+qsamp_status qsamp_set_head_wait(qsamp_ctx* c, int64_t ns) {
+    if (!c) return QSAMP_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> g(c->mu);
+    if (ns < 0) return fail(c, QSAMP_ERR_INVALID_ARG, "ns: expected >= 0, got %lld", (long long)ns);
+    c->head_wait_ns = (unsigned long long)ns;
+    return QSAMP_OK;
+}
+
 // A matrix the tensor copies read: base and rows on 16-byte boundaries.
 static qsamp_status check_matrix(qsamp_ctx* c, const char* name, const void* p, int64_t stride, int64_t least, int esz) {
     if (stride < least)
@@ -1392,6 +1401,7 @@ static qsamp_status head_call(qsamp_ctx* c, const qsamp_head* h, int grad, void*
     a.ws = (unsigned char*)workspace;
     a.num_sms = c->num_sms;
     a.status = c->head_status;
+    a.wait_ns = c->head_wait_ns;
     a.ready = &c->head_ready;
     return QSAMP_OK;
 }
@@ -1515,6 +1525,7 @@ qsamp_status qsamp_matmul_fp8(qsamp_ctx* c, const qsamp_fp8_product* p, void* st
     a.out_stride = p->out_stride;
     a.num_sms = c->num_sms;
     a.status = c->head_status;
+    a.wait_ns = c->head_wait_ns;
     a.ready = &c->head_ready;
     return on_device(c, "8-bit product launch", [&](int* n) {
         *n = 1;

@@ -62,6 +62,7 @@ struct Params {
     int slice;           // K blocks summed in tensor memory before the epilogue takes them
     int M, N;            // rows of the left and right operand
     int* status;
+    unsigned long long wait_ns;
     // LSE / DZ
     const int32_t* targets;
     float softcap;
@@ -354,7 +355,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
     cluster_sync();
     fence_after();
     const uint32_t tmem = ctl->tmem;
-    volatile int* gave_up = &ctl->gave_up;
+    const Patience patience = {&ctl->gave_up, p.status, p.wait_ns};
     launch_next();
     wait_previous();
     const uint32_t full0 = smem_addr(ctl->full), empty0 = smem_addr(ctl->empty);
@@ -369,7 +370,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
             const Job j = job_of<MODE>(p, job);
             const int m = j.m0 + rank * 128, n = j.n0 + rank * 128;
             for (int kb = 0; kb < j.k_blocks; ++kb, at.step()) {
-                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status))) break;
+                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, patience))) break;
                 if (elected()) {
                     const uint32_t full = lead_full0 + 8 * at.slot;
                     if (rank == 0) bar_expect(full0 + 8 * at.slot, 2 * STAGE_BYTES);
@@ -397,7 +398,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
         }
         // the last stages' releases arrive before this CTA may leave (a stage never used passes at once)
         for (int back = 0; ok && back < STAGES; ++back, at.step())
-            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status);
+            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, patience);
     } else if (warp == 1 && rank == 0) {
         // matrix instructions: K blocks of 128 bytes, four instructions each
         // (a barrier takes some 200 cycles to answer: the next ones are asked
@@ -417,10 +418,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
                 const bool first = left == 0;
                 if (first) left = min(p.slice, j.k_blocks - kb);
                 const bool last = --left == 0;
-                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp(full0 + 8 * at.slot, at.parity, gave_up, p.status)))
+                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp<true>(full0 + 8 * at.slot, at.parity, patience)))
                     break;
                 if (first && !__all_sync(0xffffffffu, empty) &&
-                    !(ok = bar_wait_warp(acc_empty0 + 8 * acc.slot, acc.parity ^ 1, gave_up, p.status)))
+                    !(ok = bar_wait_warp<true>(acc_empty0 + 8 * acc.slot, acc.parity ^ 1, patience)))
                     break;
                 const uint32_t slot = at.slot, buf = acc.slot;
                 at.step();
@@ -455,7 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
             unsigned char* patch = patches + (warp - 2) * OUT_PATCH;
             if constexpr (!SLICED) {
                 const float unit = *p.unit;
-                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
+                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, patience);
                 if (!ok) break;
                 fence_after();
                 if (work) grad_tile(p, j, tmem + (quarter << 21) + acc.slot * TILE + half * 128, row, half, unit, patch);
@@ -480,7 +481,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
 #pragma unroll
             for (int i = 0; i < 128; ++i) sum[i] = 0.0f;
             for (int q = 0; q < slices; ++q, acc.step()) {
-                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
+                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, patience);
                 if (!ok) break;
                 fence_after();
                 if (work) {
@@ -510,10 +511,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
         // the last boxes leave shared memory, and arrive, before the CTA does
         if (MODE != LSE && lane == 0) tma_store_wait();
     }
-    __syncwarp();
-    // a role gave up: whatever it had in flight lands while this CTA is here
-    if (*gave_up)
-        for (int i = 0; i < 20; ++i) __nanosleep(1000000);
+    let_land(patience);
     fence_before();
     cluster_sync();
     if (warp == 1) {
@@ -559,6 +557,7 @@ struct WideParams {
     CUtensorMap a, b;
     int m_tiles, n_tiles, k_blocks, jobs, M, V;
     int* status;
+    unsigned long long wait_ns;
     const float* sx;
     const float* sw;
     long long sx_stride, sw_stride, out_stride;
@@ -685,7 +684,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
     cluster_sync();
     fence_after();
     const uint32_t tmem = ctl->tmem;
-    volatile int* gave_up = &ctl->gave_up;
+    const Patience patience = {&ctl->gave_up, p.status, p.wait_ns};
 
     if (warp == 0) {
         Ring<STAGES> at;
@@ -695,7 +694,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
             int m, n;
             tile_of(job, p.m_tiles, p.n_tiles, m, n);
             for (int kb = 0; kb < p.k_blocks; ++kb, at.step()) {
-                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status))) break;
+                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, patience))) break;
                 if (elected()) {
                     const uint32_t full = lead_full0 + 8 * at.slot, da = stage0 + at.slot * STAGE_BYTES;
                     if (rank == 0) bar_expect(full0 + 8 * at.slot, 2 * STAGE_BYTES);
@@ -706,7 +705,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
             }
         }
         for (int back = 0; ok && back < STAGES; ++back, at.step())
-            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status);
+            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, patience);
     } else if (warp == 1 && rank == 0) {
         Ring<STAGES> at;
         Ring<2> acc;
@@ -715,7 +714,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
         constexpr uint32_t instr = instr_e4m3(TILE, TILE / 2);
         for (int job = pair; ok && job < p.jobs; job += pairs) {
             for (int kb = 0; ok && kb < p.k_blocks; ++kb) {
-                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp(full0 + 8 * at.slot, at.parity, gave_up, p.status)))
+                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp<true>(full0 + 8 * at.slot, at.parity, patience)))
                     break;
                 const uint32_t slot = at.slot, buf = acc.slot;
                 at.step();
@@ -724,7 +723,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (!__all_sync(0xffffffffu, empty[h]) &&
-                        !(ok = bar_wait_warp(acc_empty0 + 16 * buf + 8 * h, acc.parity ^ 1, gave_up, p.status)))
+                        !(ok = bar_wait_warp<true>(acc_empty0 + 16 * buf + 8 * h, acc.parity ^ 1, patience)))
                         break;
                     fence_after();
                     if (elected()) {
@@ -767,20 +766,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
             for (int c = 0; ok && c < chunks; ++c) {
                 const bool more = c + 1 < chunks;
                 if (more || job + pairs < p.jobs) {
-                    ok = bar_wait_warp(scales_free0 + 8 * ahead.slot, ahead.parity ^ 1, gave_up, p.status);
+                    ok = bar_wait_warp(scales_free0 + 8 * ahead.slot, ahead.parity ^ 1, patience);
                     if (!ok) break;
                     copy_scales(p, scales + ahead.slot, scales_full0 + 8 * ahead.slot, more ? job : job + pairs, rank,
                                 more ? c + 1 : 0, thread);
                     ahead.step();
                 }
-                ok = bar_wait_warp(scales_full0 + 8 * sc.slot, sc.parity, gave_up, p.status);
+                ok = bar_wait_warp(scales_full0 + 8 * sc.slot, sc.parity, patience);
                 if (!ok) break;
                 const float* xs = &scales[sc.slot].x[0][quarter * 32 + lane];
                 const float* ws = scales[sc.slot].w[block];
                 const int have = min(CHUNK, p.k_blocks - c * CHUNK);
                 for (int kb = 0; kb < have; ++kb, acc.step()) {
                     const float s = xs[kb * 128] * ws[kb];
-                    ok = bar_wait_warp(full + 16 * acc.slot, acc.parity, gave_up, p.status);
+                    ok = bar_wait_warp(full + 16 * acc.slot, acc.parity, patience);
                     if (!ok) break;
                     fence_after();
                     if (work) {
@@ -806,9 +805,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WIDE_THREADS, 1) wid
             if (ok && work) store_row64(p, sum, row, row0, col, patches + e * PATCH_ROWS * PATCH_PITCH);
         }
     }
-    __syncwarp();
-    if (*gave_up)
-        for (int i = 0; i < 20; ++i) __nanosleep(1000000);
+    let_land(patience);
     fence_before();
     cluster_sync();
     if (warp == 1) {
@@ -849,6 +846,7 @@ struct SkinnyParams {
     int V, M, k_blocks, slice, jobs;
     int tile;          // weight rows of a tile: at most 128, so that every CTA has the same number of tiles
     int* status;
+    unsigned long long wait_ns;
     const int32_t* targets;
     float softcap;
     float2* part;         // LSE: [4 CTAs][M]: a warp's maxima and sums over all its tiles
@@ -919,7 +917,7 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
     __syncthreads();
     fence_after();
     const uint32_t tmem = ctl.tmem;
-    volatile int* gave_up = &ctl.gave_up;
+    const Patience patience = {&ctl.gave_up, p.status, p.wait_ns};
     const uint32_t full0 = smem_addr(ctl.full), empty0 = smem_addr(ctl.empty);
     const uint32_t acc_full0 = smem_addr(ctl.acc_full), acc_empty0 = smem_addr(ctl.acc_empty);
     launch_next();
@@ -929,7 +927,7 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
         bool ok = true;
         for (int job = blockIdx.x; ok && job < p.jobs; job += gridDim.x) {
             for (int kb = 0; kb < p.k_blocks; ++kb, at.step()) {
-                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status))) break;
+                if (!(ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, patience))) break;
                 if (elected()) {
                     const uint32_t full = full0 + 8 * at.slot, da = stage0 + at.slot * S::STAGE;
                     bar_expect(full, p.tile * 128 + S::B_BYTES);
@@ -941,7 +939,7 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
             }
         }
         for (int back = 0; ok && back < S::DEPTH; ++back, at.step())
-            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, gave_up, p.status);
+            ok = bar_wait_warp(empty0 + 8 * at.slot, at.parity ^ 1, patience);
     } else if (warp == 1) {
         Ring<S::DEPTH> at;
         Ring<S::BUFS> acc;
@@ -954,10 +952,10 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
                 const bool first = left == 0;
                 if (first) left = min(p.slice, p.k_blocks - kb);
                 const bool last = --left == 0;
-                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp(full0 + 8 * at.slot, at.parity, gave_up, p.status)))
+                if (!__all_sync(0xffffffffu, full) && !(ok = bar_wait_warp<true>(full0 + 8 * at.slot, at.parity, patience)))
                     break;
                 if (first && !__all_sync(0xffffffffu, empty) &&
-                    !(ok = bar_wait_warp(acc_empty0 + 8 * acc.slot, acc.parity ^ 1, gave_up, p.status)))
+                    !(ok = bar_wait_warp<true>(acc_empty0 + 8 * acc.slot, acc.parity ^ 1, patience)))
                     break;
                 const uint32_t slot = at.slot, buf = acc.slot;
                 at.step();
@@ -1025,7 +1023,7 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
                     const float a = __shfl_sync(0xffffffffu, w32, kb % 32), b = __shfl_sync(0xffffffffu, w32b, kb % 32);
                     now = second ? b : a;
                 }
-                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, gave_up, p.status);
+                ok = bar_wait_warp(acc_full0 + 8 * acc.slot, acc.parity, patience);
                 if (!ok) break;
                 fence_after();
                 if (mine > 0) take<MODE, PART>(base + acc.slot * COLS, sum, table + kb * COLS + c0, now);
@@ -1092,9 +1090,7 @@ __global__ void __launch_bounds__(Skinny<MODE, COLS>::THREADS, 1) skinny_kernel(
             }
         }
     }
-    __syncwarp();
-    if (*gave_up)
-        for (int i = 0; i < 20; ++i) __nanosleep(1000000);
+    let_land(patience);
     fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -1695,6 +1691,7 @@ static cudaError_t loss_round(const HeadCall* a, int cols, bool first, int* laun
         p.k_blocks = (int)ceil_div(a->D, 64);
         p.slice = LOGIT_SKINNY_SLICE;
         p.status = a->status;
+        p.wait_ns = a->wait_ns;
         p.targets = a->targets;
         p.softcap = a->softcap;
         p.part = part;
@@ -1714,6 +1711,7 @@ static cudaError_t loss_round(const HeadCall* a, int cols, bool first, int* laun
         p.M = a->N;
         p.N = a->V;
         p.status = a->status;
+        p.wait_ns = a->wait_ns;
         p.targets = a->targets;
         p.softcap = a->softcap;
         p.part = part;
@@ -1768,6 +1766,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
         p.N = pw;
         p.n0 = p0;
         p.status = a->status;
+        p.wait_ns = a->wait_ns;
         p.unit = unit;
         if (cols) {
             SkinnyParams f = {};
@@ -1778,6 +1777,7 @@ extern "C" cudaError_t qs_head_grad(const HeadCall* a, int* launches, cudaStream
             f.k_blocks = (int)ceil_div(a->D, 64);
             f.slice = LOGIT_SKINNY_SLICE;
             f.status = a->status;
+            f.wait_ns = a->wait_ns;
             f.targets = a->targets;
             f.softcap = a->softcap;
             f.lse = a->lse;
@@ -1841,6 +1841,7 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
         p.k_blocks = (int)blocks;
         p.slice = 1;
         p.status = a->status;
+        p.wait_ns = a->wait_ns;
         p.sx = a->sx;
         p.sw = a->sw;
         p.sx_stride = a->sx_stride;
@@ -1862,6 +1863,7 @@ extern "C" cudaError_t qs_matmul_fp8(const Fp8Call* a, cudaStream_t st) {
     p.M = a->M;
     p.V = a->V;
     p.status = a->status;
+    p.wait_ns = a->wait_ns;
     p.sx = a->sx;
     p.sw = a->sw;
     p.sx_stride = a->sx_stride;

@@ -31,6 +31,7 @@ struct HeadCall {
     unsigned char* ws;
     int num_sms;
     int* status;      // mapped host word, written only when a bounded wait ran out
+    unsigned long long wait_ns;  // how long a wait may take
     uint32_t* ready;  // the context's kernels whose attributes are set
 };
 
@@ -45,6 +46,7 @@ struct Fp8Call {
     long long x_stride, w_stride, sx_stride, sw_stride, out_stride;
     int num_sms;
     int* status;
+    unsigned long long wait_ns;
     uint32_t* ready;
 };
 

@@ -69,7 +69,7 @@ EXPORTS = (
     "qsamp_trie_build", "qsamp_trie_free", "qsamp_trie_token_count", "qsamp_trie_memory_bytes",
     "qsamp_trie_collect_by_prefix", "qsamp_trie_collect_by_char_class", "qsamp_trie_collect_by_first_char",
     "qsamp_trie_mark_char_class",
-    "qsamp_head_workspace", "qsamp_head_loss", "qsamp_head_loss_grad", "qsamp_quantize_fp8", "qsamp_matmul_fp8",
+    "qsamp_set_head_wait", "qsamp_head_workspace", "qsamp_head_loss", "qsamp_head_loss_grad", "qsamp_quantize_fp8", "qsamp_matmul_fp8",
 )
 
 _P = ctypes.c_void_p
@@ -247,6 +247,8 @@ def load(path: str = LIB_PATH):
     lib.qsamp_trie_collect_by_first_char.argtypes = [_P, ctypes.c_uint8, _P, ctypes.c_int64]
     lib.qsamp_trie_mark_char_class.restype = ctypes.c_int
     lib.qsamp_trie_mark_char_class.argtypes = [_P, _P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P]
+    lib.qsamp_set_head_wait.restype = ctypes.c_int
+    lib.qsamp_set_head_wait.argtypes = [_P, ctypes.c_int64]
     lib.qsamp_head_workspace.restype = ctypes.c_int64
     lib.qsamp_head_workspace.argtypes = [_P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
     lib.qsamp_head_loss.restype = ctypes.c_int
@@ -394,8 +396,9 @@ class Context:
 
     def poll_status(self) -> None:
         """qsamp_poll_status: raises QsampError (DEVICE) when the last
-        asynchronous call's kernels hit a device-side limit; call it after
-        synchronising that call's stream."""
+        asynchronous call's kernels hit a device-side limit, or an output-head
+        kernel's did since the last report; call it after synchronising that
+        call's stream."""
         self._check(self.lib.qsamp_poll_status(self.h), "qsamp_poll_status")
 
     def limits(self) -> dict:
@@ -595,7 +598,14 @@ class Context:
 
     # ------------------------------------------------------------ output head
     # A decode step's calls here take a few microseconds of device time, so
-    # what these do on the host is kept short.
+    # what these do on the host is kept short. All are asynchronous: their
+    # results hold once the stream was synchronised and poll_status() raised
+    # nothing (a kernel whose bounded wait ran out leaves them invalid).
+    def set_head_wait(self, ns: int) -> None:
+        """qsamp_set_head_wait: the bound of the output-head kernels' waits in
+        nanoseconds (two seconds at first; 0, for tests: none is waited for)."""
+        self._check(self.lib.qsamp_set_head_wait(self.h, int(ns)), "qsamp_set_head_wait")
+
     def _empty(self, stream, shape, dtype):
         """An uninitialised tensor on this context's device, for use on
         `stream` (None: torch's current stream), from whose memory it comes."""
