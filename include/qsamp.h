@@ -335,7 +335,10 @@ qsamp_status qsamp_verify_greedy(qsamp_ctx* ctx, const void* logits, qsamp_dtype
  * written), whatever its hidden row holds, NaN included; a target >= V gives
  * loss NaN and no gradient. -loss is the
  * token's log-probability (logprobs of generated tokens, prompt scoring).
- * A logit of +infinity or NaN makes its row's results NaN.
+ * A logit of +infinity or NaN makes its row's results NaN. Products and
+ * sums are held in 32 bits; the tensor cores cut the last bits of a sum's
+ * additions, so that an lse is low by some 1e-6 of it or less. A soft-cap of
+ * up to 64 is applied with an absolute error of a few 2^-24 of it.
  *
  * qsamp_head_loss_grad takes the lse of the forward call on the same inputs
  * and grad_loss[n] = d(total) / d(loss[n]):
@@ -367,8 +370,9 @@ typedef struct qsamp_head {
     float softcap;           /* 0: off; 2^-60 to 2^60            */
 } qsamp_head;
 /* The bound of the waits in the output-head kernels launched from now on, in
- * nanoseconds (a captured graph keeps its own); 0 (tests): the matrix
- * instructions do not wait for the first operands, and all else runs out. */
+ * nanoseconds; 0 (tests): the matrix instructions do not wait for the first
+ * operands, and all other waits run out. A captured graph keeps the bound it
+ * was captured with and reports to its context, which has to outlive it. */
 qsamp_status qsamp_set_head_wait(qsamp_ctx* ctx, int64_t ns);
 int64_t qsamp_head_workspace(const qsamp_ctx* ctx, int32_t N, int32_t V, int32_t D, int32_t grad);
 qsamp_status qsamp_head_loss(qsamp_ctx* ctx, const qsamp_head* head, float* out_loss, float* out_lse, void* workspace,
@@ -391,8 +395,9 @@ qsamp_status qsamp_head_loss_grad(qsamp_ctx* ctx, const qsamp_head* head, const 
  *   x_scale[m][kb] * w_scale[n / 128][kb] * (x[m] . w[n] within the block),
  * x [M][x_stride] with a scale per row and block, w [V][w_stride] with a scale
  * per 128 x 128 block: the head's logits for qsamp_sample (or any linear
- * layer). Products within a block and the sum over blocks are held in 32
- * bits; out is fp32 or bf16, rounded once. x and w 16-byte aligned with
+ * layer). Products within a block, the product of the two scales (0 or in
+ * fp32's normal range, else its digits are lost) and the sum over blocks are held in 32 bits;
+ * out is fp32 or bf16, rounded once. x and w 16-byte aligned with
  * strides a multiple of 16 (else QSAMP_ERR_UNSUPPORTED); K, M and V any size;
  * out any alignment of its type and any stride >= V. */
 typedef struct qsamp_fp8_product {

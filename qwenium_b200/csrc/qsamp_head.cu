@@ -12,11 +12,12 @@
 // The pair halves what each SM loads per flop: 32 KB per 512 tensor cycles
 // instead of 48 KB, which the L2 could not feed to 148 SMs.
 //
-// Measured (4096 x 2048 x 151936, one launch at full clock): loss 1.57 ms = 1.62
-// PFLOP/s, dz of five pieces 1.55 ms, gradients 3.2 ms = 1.58 PFLOP/s; the
-// tensor pipe is 74 to 78% active. In a loop the 1000 W limit sets the pace
-// (8.0 ms a step, 1.17 GHz): 91% of cuBLAS's sustained rate over the 8 N D V
-// operations, a quarter of them the logits made a second time.
+// Measured (4096 x 2048 x 32768, single launches): loss 342 us = 1.61 PFLOP/s,
+// tensor pipe 88% active; dz 384 us = 1.43 PFLOP/s, 78%; gradients 710 us = 1.55
+// PFLOP/s, 87%. At a depth of 1152, with a soft-cap, the epilogues set the pace
+// (45% and 38% in loss and dz). In a loop at 4096 x 2048 x 151936 the 1000 W
+// limit does (8.1 ms a step, 1.3 GHz): 90% of cuBLAS's sustained rate over the
+// 8 N D V operations, a quarter of them the logits made a second time.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -525,12 +526,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) head_ker
 // The block-scaled product of many rows. Scales differ from K block to K
 // block, so each block's sums leave tensor memory after four instructions and
 // are added up in registers: a round trip (instructions, signal, read, signal
-// back) per two blocks, which sets the pace with the power limit. What shortens
-// it: sixteen epilogue warps of 64 columns each (four loads and 32 packed fmas
-// a block), accumulators handed over in halves of 128 columns, so that one
-// half is read while the other is filled, and scales brought to shared memory
-// by asynchronous copies 16 K blocks ahead (read from global memory they cost
-// 800 cycles a block). Measured: 256 x 4096 x 151936 in 223 us (tensor pipe 36%
+// back) per two blocks, which sets the pace: no pipe is full (below), and the
+// power limit adds a seventh in a loop. What shortens it: sixteen epilogue
+// warps of 64 columns each (four loads and 32 packed fmas a block), accumulators
+// handed over in halves of 128 columns, so that one half is read while the other
+// is filled, and scales brought to shared memory by asynchronous copies 16 K
+// blocks ahead (read from global memory they cost 800 cycles a block).
+// Measured: 256 x 4096 x 151936 in 223 us (tensor pipe 36%
 // active, 1.00x of the bytes), 255 in a loop at 1.58 GHz; 4096 x 4048 x 16384 in
 // 350 us = 1.55 PFLOP/s.
 constexpr int WIDE_EPI = 16;
@@ -1352,10 +1354,12 @@ __device__ __forceinline__ void store8(uint8_t* row, int k, int K, bool vec, uin
 // pieces, so that a load's lanes are neighbours); a warp takes 512 columns of
 // four rows with all their loads in flight. Each value is read once and held
 // in registers between the maximum and the quotients (8000 x 8192 bf16 in 38
-// us = 5.1 TB/s, its instructions' rate; the square blocks' kernel 151936 x
-// 4096 in 277 us = 6.7 TB/s). FULL: whole blocks and whole groups of rows on aligned addresses, without checks per value (which
-// would cost registers, and a quarter of the rate). A CTA's warps lie below
-// each other, so that the few slower ones at the right edge share CTAs.
+// us = 5.1 TB/s; neither memory, 49% of its peak, nor issue, 56%, is full: a
+// warp's loads and its arithmetic take turns, with three CTAs an SM; the square
+// blocks' kernel 151936 x 4096 in 277 us = 6.7 TB/s). FULL: whole blocks and
+// whole groups of rows on aligned addresses, without checks per value (which
+// would cost registers, and a quarter of the rate). A CTA's warps lie below each
+// other, so that the few slower ones at the right edge share CTAs.
 constexpr int QROWS = 4, QCOLS = 512;
 struct QuantArgs {
     const void* x;
@@ -1591,7 +1595,8 @@ cudaError_t launch_skinny(int cols, SkinnyParams& p, const void* weight, long lo
 // slices a target of loss 1e-5 had dz -4e-4 at D 4160, -9.6e-4 at D 8192.) Shorter
 // slices are free where the weight's bytes bound the kernel; the pair's loss
 // takes 2% more at 8 than at 16, 13% at 4; the pair's dz against one slice:
-// 509 x 1152 x 50021 256 against 238 us a step, 4096 x 2048 x 151936 7.94 against 7.82 ms.
+// 509 x 1152 x 50021 76 against 59 us (a step 260 against 245), 4096 x 2048 x
+// 151936 1% of a step.
 constexpr int LOGIT_SLICE = 8, LOGIT_SKINNY_SLICE = 2;
 // The gradients' sums, over the rows (d_weight) and over a split of the
 // vocabulary (d_hidden), stay in tensor memory for at most 32768 products. A sum

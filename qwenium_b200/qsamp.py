@@ -669,6 +669,7 @@ class Context:
         """qsamp_head_loss on CUDA tensors: hidden bf16 [N][D], weight bf16
         [V][D], targets int32 [N] (negative: no loss for the row). Returns
         (loss, lse) float32 [N]; -loss is each target's log-probability.
+        Asynchronous; valid once poll_status raised nothing.
         `stream`: a raw stream handle (default: torch's current stream)."""
         import torch
 
@@ -683,7 +684,8 @@ class Context:
                        d_weight=None, stream=None):
         """qsamp_head_loss_grad on CUDA tensors: the inputs of head_loss, its
         lse, and grad_loss float32 [N] = d(total) / d(loss). Returns
-        (d_hidden, d_weight) bf16, written into the given tensors if any."""
+        (d_hidden, d_weight) bf16, written into the given tensors if any.
+        Asynchronous; valid once poll_status raised nothing."""
         import torch
 
         h = self._head(hidden, weight, targets, softcap)
@@ -724,7 +726,8 @@ class Context:
         """qsamp_matmul_fp8 on CUDA tensors: x float8_e4m3fn [M][K] with
         x_scale float32 [M][ceil(K/128)], w float8_e4m3fn [V][K] with w_scale
         float32 [ceil(V/128)][ceil(K/128)]. Returns out [M][V], bfloat16
-        unless `out` or `out_dtype` says float32."""
+        unless `out` or `out_dtype` says float32. Asynchronous; valid once
+        poll_status raised nothing."""
         import torch
 
         M, K = self._tensor("x", x, (torch.float8_e4m3fn,), (None, None))
