@@ -337,8 +337,9 @@ qsamp_status qsamp_verify_greedy(qsamp_ctx* ctx, const void* logits, qsamp_dtype
  * token's log-probability (logprobs of generated tokens, prompt scoring).
  * A logit of +infinity or NaN makes its row's results NaN. Products and
  * sums are held in 32 bits; the tensor cores cut the last bits of a sum's
- * additions, so that an lse is low by some 1e-6 of it or less. A soft-cap of
- * up to 64 is applied with an absolute error of a few 2^-24 of it.
+ * additions, so that an lse is low by some 4e-6, or 1e-6 of the largest logit
+ * (up to 64 rows: a quarter of that). A soft-cap of up to 64 is applied with
+ * an absolute error of a few 2^-24 of it.
  *
  * qsamp_head_loss_grad takes the lse of the forward call on the same inputs
  * and grad_loss[n] = d(total) / d(loss[n]):
@@ -396,8 +397,8 @@ qsamp_status qsamp_head_loss_grad(qsamp_ctx* ctx, const qsamp_head* head, const 
  * x [M][x_stride] with a scale per row and block, w [V][w_stride] with a scale
  * per 128 x 128 block: the head's logits for qsamp_sample (or any linear
  * layer). Products within a block, the product of the two scales (0 or in
- * fp32's normal range, else its digits are lost) and the sum over blocks are held in 32 bits;
- * out is fp32 or bf16, rounded once. x and w 16-byte aligned with
+ * fp32's normal range, else its digits are lost) and the sum over blocks are
+ * held in 32 bits; out is fp32 or bf16, rounded once. x and w 16-byte aligned with
  * strides a multiple of 16 (else QSAMP_ERR_UNSUPPORTED); K, M and V any size;
  * out any alignment of its type and any stride >= V. */
 typedef struct qsamp_fp8_product {
